@@ -723,6 +723,110 @@ typedef struct {
 } M40llmMoe;
 int m40llm_moe_async(M40llmCudaContext* ctx, const M40llmMoe* call, uint32_t stream_kind);
 
+/* ---------------------------------------------------------------------
+ * A key / value cache in pages (no counterpart in the reference). The pool and the page table belong to the caller, so memory
+ * follows what the sequences hold, pages can be shared between slots for reading, and freeing a sequence is a host's matter.
+ *   k, v   elem_dtype (M40LLM_DT_F16 or M40LLM_DT_F32) [pages][kv_heads][page_tokens][head_dim]
+ *   table  device [slots][max_pages]: the page of entries i * page_tokens .. of a slot
+ * An entry is a place in a slot's list; attention does not depend on the entries' order, so an entry's position is kept apart
+ * where it is needed (entry_pos, below). page_tokens is a power of two up to 4096, head_dim at most 512, a slot has at most 2^30
+ * entries; pointers are aligned to their elements (16-byte alignment of k and v is faster). Decode stream. Every call returns
+ * -1 for a null argument, -2 for a size that does not fit, -4 for a type, -3 when the launch failed, -5 without scratch,
+ * M40LLM_ERR_LIMIT beyond a limit. Rows with a slot or an entry outside the cache, and pages outside the pool, touch no memory:
+ * status bit 2 where something was to be written, bit 1 where it was to be read. */
+typedef struct {
+    void* k;
+    void* v;
+    const uint32_t* table;
+    uint32_t pages, page_tokens, slots, max_pages, kv_heads, head_dim, elem_dtype;
+} M40llmPagedCache;
+
+/* Appends one token per row: k and v f32 rows [kv_heads * head_dim] go to entry row_entry[r] of slot row_slot[r]. With pairs > 0
+ * the first 2 * pairs dimensions of every head of k (and of q, which goes to q_out f32 [rows][q_heads * head_dim]) turn by
+ * row_pos[r] * turns[m] full turns, pair m being (m, m + pairs) for rope_layout 1 and (2 m, 2 m + 1) for 0; turns f64 [pairs] as in
+ * M40llmRotaryAttention. ld is the row pitch of q, k and v in elements (0: each its own width), so that they may be parts of one
+ * packed projection; q_out may be q where ld is 0. entry_pos u32 and weights f32, both [slots][kv_heads][ld_entry] or null: the new
+ * entry gets its position and the weight 0. row_pos may be null where neither pairs nor entry_pos need it, q where q_heads is 0. Two
+ * rows of a call name different entries; what an entry named twice holds is one or the other, element by element. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    const void* turns;
+    const uint32_t* row_slot;
+    const uint32_t* row_entry;
+    const uint32_t* row_pos;
+    uint32_t* entry_pos;
+    void* weights;
+    uint32_t rows, ld, q_heads, pairs, rope_layout, ld_entry;
+} M40llmPagedAppend;
+int m40llm_paged_append_async(M40llmCudaContext* ctx, const M40llmPagedCache* cache, const M40llmPagedAppend* call);
+
+/* Attention of single tokens: out[r] = softmax(scale * q[r] . k) v per q head over the entries row_begin[r] (null: 0) .. row_len[r] - 1 of
+ * slot row_slot[r]; q and out f32 [rows][q_heads * head_dim]. A row without entries gives zeros. max_len: a bound of row_len that the
+ * work is dealt by (0: the capacity; a row beyond it is one outside the cache).
+ * With weights_out f32 [slots][kv_heads][ld_weights]: entry e of a slot that has rows in the call, e below the largest row_len of
+ * these, gets weights_in[...][e] (null: 0; may be weights_out itself) + the softmax weights that these rows gave it, summed over the q heads of its kv
+ * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. */
+typedef struct {
+    const void* q;
+    void* out;
+    const uint32_t* row_slot;
+    const uint32_t* row_len;
+    const uint32_t* row_begin;
+    const void* weights_in;
+    void* weights_out;
+    uint32_t rows, q_heads, ld_weights, max_len;
+    float scale;
+} M40llmPagedAttention;
+int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llmPagedCache* cache, const M40llmPagedAttention* call);
+
+/* Keeps the `keep` best of the first len[i] entries of slot seq[i], per kv head: entries whose position is below `first` or among the
+ * `recent` newest positions (newest - position < recent) come before any other (entry_pos null: positions are entries), the others by
+ * weight (NaN below all else); the lower entry first where that leaves a choice. Kept entries below the new length stay where they are; the
+ * places of the others there are taken, in ascending order, by the kept ones from behind the new end. origin u32 [count][kv_heads][keep] (or null) says where each entry came from (0xffffffff beyond the new length),
+ * new_len u32 [count] = min(len, keep). `to` null: in place, only what moves is copied; it may hold pages that no other slot
+ * reads. Otherwise the kept entries go to the same slots of `to`, a cache of the same heads, size and type on other pages. weights_out and
+ * entry_pos_out [slots][kv_heads][ld] take the kept entries' values (null: not kept; the arrays themselves: in place).
+ * max_len bounds len (0: the capacity). A slot outside the cache or named before in seq, or a length beyond max_len, keeps nothing: new_len 0. */
+typedef struct {
+    const M40llmPagedCache* to;
+    const uint32_t* seq;
+    const uint32_t* len;
+    const void* weights;
+    void* weights_out;
+    const uint32_t* entry_pos;
+    uint32_t* entry_pos_out;
+    uint32_t* origin;
+    uint32_t* new_len;
+    uint32_t count, keep, first, recent, ld, max_len;
+} M40llmPagedEvict;
+int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cache, const M40llmPagedEvict* call);
+
+/* Log probabilities of f32 logits [rows][ld] (ld 0 = n): with lse the log of the sum of exp over a row's n values,
+ *   logprob f32 [rows]        logits[tokens[r]] - lse,
+ *   rank u32 [rows]           1 + the values that come before it (larger, or equal at a lower index),
+ *   entropy f32 [rows]        lse - sum of p * logits, p = exp(logits - lse),
+ *   lse f32 [rows],
+ *   top_ids u32 / top_logprobs f32 [rows][top]   the `top` <= 64 most likely, descending, ties to the lower index.
+ * Any output may be null; tokens too where logprob and rank are. NaN counts as -inf, as it does for the greedy choice; values of -inf
+ * have probability 0 and are never listed (0xffffffff, -inf in their place). Where a row holds +inf, these share the
+ * probability. A row without any value above -inf: entropy 0, lse and logprobs -inf. A token >= n: status bit 8, logprob -inf, rank 0. Decode stream; return
+ * codes as above. */
+typedef struct {
+    const void* logits;
+    const uint32_t* tokens;
+    void* logprob;
+    uint32_t* rank;
+    void* entropy;
+    void* lse;
+    uint32_t* top_ids;
+    void* top_logprobs;
+    uint32_t rows, n, ld, top;
+} M40llmLogprobs;
+int m40llm_logprobs_f32_async(M40llmCudaContext* ctx, const M40llmLogprobs* call);
+
 /* Token embedding gather for any table type (M40LLM_DT_*); an id >= vocab as in m40llm_embed_tokens_f16_async. */
 int m40llm_embed_tokens_async(M40llmCudaContext* ctx, const void* d_table, uint32_t table_dtype,
                               const uint32_t* d_token_ids, void* d_out_f32, uint32_t rows, uint32_t hidden,

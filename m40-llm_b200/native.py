@@ -83,6 +83,37 @@ class Moe(C.Structure):
                                           "w_dtype", "act", "exact")] + [("scale", C.c_float)])
 
 
+class PagedCache(C.Structure):
+    """M40llmPagedCache."""
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "table")] +
+                [(n, C.c_uint32) for n in ("pages", "page_tokens", "slots", "max_pages", "kv_heads", "head_dim", "elem_dtype")])
+
+
+class PagedAppend(C.Structure):
+    """M40llmPagedAppend."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "turns", "row_slot", "row_entry", "row_pos", "entry_pos", "weights")] +
+                [(n, C.c_uint32) for n in ("rows", "ld", "q_heads", "pairs", "rope_layout", "ld_entry")])
+
+
+class PagedAttention(C.Structure):
+    """M40llmPagedAttention."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "out", "row_slot", "row_len", "row_begin", "weights_in", "weights_out")] +
+                [(n, C.c_uint32) for n in ("rows", "q_heads", "ld_weights", "max_len")] + [("scale", C.c_float)])
+
+
+class PagedEvict(C.Structure):
+    """M40llmPagedEvict."""
+    _fields_ = ([(n, C.c_void_p) for n in ("to", "seq", "len", "weights", "weights_out", "entry_pos", "entry_pos_out", "origin",
+                                          "new_len")] +
+                [(n, C.c_uint32) for n in ("count", "keep", "first", "recent", "ld", "max_len")])
+
+
+class Logprobs(C.Structure):
+    """M40llmLogprobs."""
+    _fields_ = ([(n, C.c_void_p) for n in ("logits", "tokens", "logprob", "rank", "entropy", "lse", "top_ids", "top_logprobs")] +
+                [(n, C.c_uint32) for n in ("rows", "n", "ld", "top")])
+
+
 _SCALARS = {
     "int": C.c_int, "uint32_t": C.c_uint32, "uint64_t": C.c_uint64, "size_t": C.c_size_t, "float": C.c_float,
 }
