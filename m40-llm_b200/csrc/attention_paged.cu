@@ -3,6 +3,7 @@
 // Work is dealt as (row, kv head, chunk of entries): softmax statistics are kept with a running maximum in base 2, and the chunks'
 // (maximum, sum, unnormalised output) meet in paged_merge_kernel in a fixed order. Where accumulated weights are asked for, the
 // scores are kept in scratch and paged_weights_kernel turns them into weights once the maximum and sum of every row are known.
+//   paged_tiles_kernel  f16 entries, head sizes 64 and 128: matrix instructions on 64-entry tiles
 //   paged_rows_kernel   any head size, group size and type: f32 multiply-adds on tiles in shared memory
 #include "attention_mma.cuh"
 #include "paged.cuh"
@@ -220,39 +221,373 @@ __global__ void __launch_bounds__(ROWS_THREADS) paged_rows_kernel(PagedAttnArgs 
         }
 }
 
-// CTA = (q head, row): the chunks' parts in order.
-__global__ void __launch_bounds__(128) paged_merge_kernel(PagedAttnArgs a) {
-    __shared__ float red[8];
+// One q head over the entries [t0, t1) of one kv head in plain f32, by one warp: what the matrix instructions cannot give where keys or values are
+// not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions 2 lane, 2 lane + 1 (+ 64). Scale as in PagedAttnArgs.
+template <int HD>
+__device__ __noinline__ void paged_plain_head(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
+                                              uint32_t t1, float bias, float* m_out, float* l_out, float* o_out) {
+    const uint32_t lane = threadIdx.x & 31u, d = 2u * lane;
+    const __half* K = reinterpret_cast<const __half*>(a.c.k);
+    const __half* V = reinterpret_cast<const __half*>(a.c.v);
+    float x[HD / 32], o[HD / 32], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j) {
+        x[2 * j] = q[d + 64 * j] * a.scale, x[2 * j + 1] = q[d + 64 * j + 1] * a.scale;
+        o[2 * j] = o[2 * j + 1] = 0.0f;
+    }
+    for (uint32_t e = t0; e < t1; ++e) {
+        const uint32_t page = paged_page(a.c, slot, e);
+        if (page == PAGED_NONE) continue;
+        const size_t at = paged_row(a.c, page, kvh, e) + d;
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            const float2 k = __half22float2(*reinterpret_cast<const __half2*>(K + at + 64 * j));
+            s += x[2 * j] * k.x + x[2 * j + 1] * k.y;
+        }
+        s = warp_sum(s);
+        if (scores && lane == 0) scores[e] = s;
+        const float m_new = fmaxf(m, s - bias), use = m_new == -INFINITY ? 0.0f : m_new;
+        const float corr = m == -INFINITY ? 0.0f : exp2f(m - m_new), p = exp2f(s - use);
+        l = l * corr + p;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(V + at + 64 * j));
+            o[2 * j] = o[2 * j] * corr + p * v.x, o[2 * j + 1] = o[2 * j + 1] * corr + p * v.y;
+        }
+        m = m_new;
+    }
+    if (lane == 0) *m_out = m, *l_out = l;
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j) o_out[d + 64 * j] = o[2 * j], o_out[d + 64 * j + 1] = o[2 * j + 1];
+}
+
+// 16 bytes by cp.async; zeros where `bytes` is 0 (the source is then not read)
+__device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, uint32_t bytes) {
+    const uint32_t s = (uint32_t)__cvta_generic_to_shared(smem);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(gmem), "r"(bytes));
+}
+
+constexpr uint32_t TILE = 64, TILES_THREADS = 128;
+// Weights are relative to the maximum less 15: f16 then holds a small one down to 2^-40 of the largest instead of 2^-25. That reference, as it is
+// rounded, is what a part carries as its maximum.
+constexpr float WEIGHT_BIAS = 15.0f;
+
+// CTA = (row, up to 8 (WIDE: 16) q heads of one kv head, chunk). K and V tiles of 64 entries come through a ring of cp.async stages, rows
+// looked up in the page table as they are fetched, into XOR-swizzled shared memory; a warp takes 16 entries of a tile.
+//   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them. A group has
+//                         at most 8 heads as a rule: hi and lo are then the two halves of the 16 rows of ONE operand, and the halves of the result are
+//                         added (WIDE: two products).
+//   softmax               online in base 2 per warp; the outputs are rescaled only when a maximum moved.
+// Two CTAs per SM with 96 (64) KB of ring each; bound by HBM for long chunks.
+template <int HD, bool WIDE>
+__global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttnArgs a, uint32_t per) {
+    constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = HD == 128 ? 3 : 4, ROWS = WIDE ? 16 : 8;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint32_t s_bad;
+    __half* sK = reinterpret_cast<__half*>(smem);
+    __half* sV = sK + STAGES * TILE * HD;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
+    if (tid == 0) s_bad = 0u;
     pdl_wait();
     pdl_trigger();
-    const uint32_t tid = threadIdx.x, hd = a.c.hd;
-    const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
-    float M = -INFINITY, nan = 0.0f;
-    for (uint32_t s = tid; s < a.splits; s += 128u) {
-        const float l = a.part_l[base + s];
-        if (l != 0.0f) M = fmaxf(M, a.part_m[base + s]);
-        if (isnan(l)) nan = 1.0f;
+    const uint32_t split = blockIdx.x, row = blockIdx.z, subgroups = (a.group + per - 1) / per;
+    const uint32_t kvh = blockIdx.y / subgroups, g0 = (blockIdx.y % subgroups) * per, G = min(per, a.group - g0), head0 = kvh * a.group + g0;
+    uint32_t slot, begin, end, t0 = 0, t1 = 0;
+    const bool inside = paged_row_range(a, row, &slot, &begin, &end);
+    if (!inside && tid == 0 && split == 0 && blockIdx.y == 0) atomicOr(a.status, 1u);
+    if (inside) paged_chunk(a, split, begin, end, &t0, &t1);
+    const bool partial = a.splits > 1 || a.scores;
+    if (t0 >= t1) {  // nothing in this chunk: an empty part (l = 0), or the row's zeros
+        for (uint32_t i = tid; i < G; i += TILES_THREADS)
+            if (partial) {
+                const size_t pi = ((size_t)row * a.q_heads + head0 + i) * a.splits + split;
+                a.part_m[pi] = -INFINITY;
+                a.part_l[pi] = 0.0f;
+            }
+        if (!partial)
+            for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) a.out[((size_t)row * a.q_heads + head0) * HD + i] = 0.0f;
+        return;
     }
-    M = warp_max(M);
-    nan = warp_max(nan);
-    if ((tid & 31u) == 0) red[tid >> 5] = M, red[4 + (tid >> 5)] = nan;
     __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float L = 0.0f;
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float l = a.part_l[base + s];
-        if (l != 0.0f) L += l * exp2f(a.part_m[base + s] - M);
-    }
-    const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : NAN);
-    for (uint32_t d = tid; d < hd; d += 128u) {
-        float o = 0.0f;
-        for (uint32_t s = 0; s < a.splits; ++s) {
-            const float l = a.part_l[base + s];
-            if (l != 0.0f) o = fmaf(exp2f(a.part_m[base + s] - M), a.part_o[(base + s) * hd + d], o);
+    const uint32_t n_tiles = (t1 - t0 + TILE - 1) / TILE;
+    const __half* K = reinterpret_cast<const __half*>(a.c.k);
+    const __half* V = reinterpret_cast<const __half*>(a.c.v);
+    const uint32_t* pages = a.c.table + (size_t)slot * a.c.max_pages;
+    const uint32_t in_page = (1u << a.c.shift) - 1u;
+    auto load = [&](uint32_t tile) {
+        const uint32_t base = t0 + tile * TILE, stage = tile % STAGES, ch = tid % CHUNKS;
+        uint32_t page[TILE * CHUNKS / TILES_THREADS];
+#pragma unroll
+        for (int c = 0; c < (int)(TILE * CHUNKS / TILES_THREADS); ++c) {  // all lookups on their way together
+            const uint32_t e = base + c * (TILES_THREADS / CHUNKS) + tid / CHUNKS;
+            page[c] = e < t1 ? pages[e >> a.c.shift] : PAGED_NONE;
         }
-        a.out[head * hd + d] = L == 0.0f ? 0.0f : o * inv;
+#pragma unroll
+        for (int c = 0; c < (int)(TILE * CHUNKS / TILES_THREADS); ++c) {
+            const uint32_t r = c * (TILES_THREADS / CHUNKS) + tid / CHUNKS, e = base + r;
+            const bool ok = page[c] < a.c.pages;
+            if (!ok && e < t1) s_bad = 1u;
+            const size_t src = ok ? ((((size_t)page[c] * a.c.kv_heads + kvh) << a.c.shift) + (e & in_page)) * HD + ch * 8u : 0;
+            const uint32_t dst = stage * TILE * HD + r * HD + ((ch ^ (r & 7u)) * 8u);
+            cp_async16_or_zero(sK + dst, K + src, ok ? 16u : 0u);
+            cp_async16_or_zero(sV + dst, V + src, ok ? 16u : 0u);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        if ((uint32_t)s < n_tiles) load(s);
+        cp_async_commit();
     }
-    if (a.stat && tid == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = inv;
+
+    // A operand of the scores: rows 0-7 hi, 8-15 lo of heads 0-7; WIDE: rows are heads, hi and lo apart
+    uint32_t qa[KS][4], qb[WIDE ? KS : 1][4];
+    {
+        const float* q0 = a.q + ((size_t)row * a.q_heads + head0 + g) * HD;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t k0 = ks * 16 + half * 8 + 2 * t4;
+                const float x = g < G ? q0[k0] * a.scale : 0.0f, y = g < G ? q0[k0 + 1] * a.scale : 0.0f;
+                uint32_t hi, lo;
+                split_h2(x, y, &hi, &lo);
+                qa[ks][2 * half] = hi;
+                if (WIDE) {
+                    qb[ks][2 * half] = lo;
+                    const float* q1 = q0 + 8 * HD;
+                    const float u = g + 8u < G ? q1[k0] * a.scale : 0.0f, w = g + 8u < G ? q1[k0 + 1] * a.scale : 0.0f;
+                    split_h2(u, w, &qa[ks][2 * half + 1], &qb[ks][2 * half + 1]);
+                } else {
+                    qa[ks][2 * half + 1] = lo;
+                }
+            }
+    }
+    float o[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    constexpr int H = WIDE ? 2 : 1;  // heads of a thread
+    float m_run[H], l_run[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
+
+    for (uint32_t tile = 0; tile < n_tiles; ++tile) {
+        cp_async_wait<STAGES - 2>();
+        __syncthreads();
+        if (tile + STAGES - 1 < n_tiles) load(tile + STAGES - 1);
+        cp_async_commit();
+        const __half* tK = sK + (size_t)(tile % STAGES) * TILE * HD;
+        const __half* tV = sV + (size_t)(tile % STAGES) * TILE * HD;
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+            const uint32_t j = lane >> 3, r = warp * 16 + (j >> 1) * 8 + (lane & 7u);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t ch = ks * 2 + (j & 1u);
+                uint32_t b[4];
+                ldmatrix_x4(b, tK + r * HD + ((ch ^ (r & 7u)) * 8));
+                mma16816(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+                mma16816(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+                if (WIDE) {
+                    mma16816(s0, qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[0], b[1]);
+                    mma16816(s1, qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[2], b[3]);
+                }
+            }
+        }
+        // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
+        const uint32_t e0 = t0 + tile * TILE + warp * 16 + 2 * t4;
+        float s[H][4];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            s[h][0] = WIDE ? s0[2 * h] : s0[0] + s0[2], s[h][1] = WIDE ? s0[2 * h + 1] : s0[1] + s0[3];
+            s[h][2] = WIDE ? s1[2 * h] : s1[0] + s1[2], s[h][3] = WIDE ? s1[2 * h + 1] : s1[1] + s1[3];
+        }
+        const bool bad = *(volatile uint32_t*)&s_bad != 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
+            const bool out = e >= t1 || (bad && pages[e >> a.c.shift] >= a.c.pages);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                if (out) s[h][i] = -INFINITY;
+                if (a.scores && g + 8u * h < G && e < t1) a.scores[((size_t)row * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
+            }
+        }
+        uint32_t ph[H][2], pl[H][2];
+        bool moved = false;
+        float corr[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            float mx = fmaxf(fmaxf(s[h][0], s[h][1]), fmaxf(s[h][2], s[h][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_run[h], mx - WEIGHT_BIAS), use = m_new == -INFINITY ? 0.0f : m_new;
+            moved |= m_new > m_run[h];
+            corr[h] = fast_exp2(m_run[h] - use);
+            const float p0 = fast_exp2(s[h][0] - use), p1 = fast_exp2(s[h][1] - use);
+            const float p2 = fast_exp2(s[h][2] - use), p3 = fast_exp2(s[h][3] - use);
+            l_run[h] = l_run[h] * corr[h] + ((p0 + p1) + (p2 + p3));  // this thread's entries; the quad's sums meet at the end
+            m_run[h] = m_new;
+            split_h2(p0, p1, &ph[h][0], &pl[h][0]);
+            split_h2(p2, p3, &ph[h][1], &pl[h][1]);
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                o[n][0] *= corr[0], o[n][1] *= corr[0];
+                o[n][2] *= corr[H - 1], o[n][3] *= corr[H - 1];
+            }
+        }
+        {
+            const uint32_t j = lane >> 3, r = warp * 16 + (j & 1u) * 8 + (lane & 7u);
+#pragma unroll
+            for (int nd = 0; nd < HD / 16; ++nd) {
+                const uint32_t ch = nd * 2 + (j >> 1);
+                uint32_t b[4];
+                ldmatrix_x4_trans(b, tV + r * HD + ((ch ^ (r & 7u)) * 8));
+                if (WIDE) {
+                    mma16816(o[2 * nd], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[0], b[1]);
+                    mma16816(o[2 * nd + 1], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[2], b[3]);
+                    mma16816(o[2 * nd], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[0], b[1]);
+                    mma16816(o[2 * nd + 1], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[2], b[3]);
+                } else {
+                    mma16816(o[2 * nd], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[0], b[1]);
+                    mma16816(o[2 * nd + 1], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[2], b[3]);
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+
+    // the four warps' parts through shared memory, over the ring that is done with
+    float* sm_m = reinterpret_cast<float*>(smem);  // [4][ROWS]
+    float* sm_l = sm_m + 4 * ROWS;                 // [4][ROWS]
+    float* sm_o = sm_l + 4 * ROWS;                 // [4][ROWS][HD], then the heads' own [ROWS][HD]
+    float* sm_r = sm_o + 4 * ROWS * HD;
+    float* sm_t = sm_r + ROWS * HD;                // [ROWS][2]: m, l of the heads
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        float l = l_run[h];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t4 == 0) sm_m[warp * ROWS + g + 8 * h] = m_run[h], sm_l[warp * ROWS + g + 8 * h] = l;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float* dst = sm_o + ((size_t)warp * ROWS + g) * HD + n * 8 + 2 * t4;
+        if (WIDE) {
+            dst[0] = o[n][0], dst[1] = o[n][1];
+            dst[8 * HD] = o[n][2], dst[8 * HD + 1] = o[n][3];
+        } else {
+            dst[0] = o[n][0] + o[n][2], dst[1] = o[n][1] + o[n][3];
+        }
+    }
+    __syncthreads();
+    if (s_bad && tid == 0) atomicOr(a.status, 1u);
+    // a warp finishes a head at a time
+    for (uint32_t h = warp; h < G; h += 4u) {
+        float M = -INFINITY, L = 0.0f, e[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w * ROWS + h]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = sm_m[w * ROWS + h], lw = sm_l[w * ROWS + h];
+            e[w] = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - M);
+            L += lw * e[w];
+        }
+        bool fine = is_finite(L);
+        for (uint32_t d = lane; d < HD; d += 32u) {
+            float O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) O += sm_o[((size_t)w * ROWS + h) * HD + d] * e[w];
+            sm_r[h * HD + d] = O;
+            fine &= is_finite(O);
+        }
+        const size_t head = (size_t)row * a.q_heads + head0 + h;
+        if (!__all_sync(0xffffffffu, fine)) {
+            paged_plain_head<HD>(a, slot, kvh, a.q + head * HD, a.scores ? a.scores + head * a.ld_scores : nullptr, t0, t1, WEIGHT_BIAS, sm_t + 2 * h,
+                                 sm_t + 2 * h + 1, sm_r + h * HD);
+            __syncwarp();
+            M = sm_t[2 * h], L = sm_t[2 * h + 1];
+        }
+        __syncwarp();
+        if (partial) {
+            if (lane == 0) a.part_m[head * a.splits + split] = M, a.part_l[head * a.splits + split] = L;
+            for (uint32_t d = lane; d < HD; d += 32u) a.part_o[(head * a.splits + split) * HD + d] = sm_r[h * HD + d];
+        } else {
+            for (uint32_t d = lane; d < HD; d += 32u) a.out[head * HD + d] = L == 0.0f ? 0.0f : sm_r[h * HD + d] / L;
+        }
+    }
+}
+
+// CTA = (q head, row): the chunks' parts in order. Thread s has chunk s's weight (at most 256 chunks); then eight groups of lanes take every eighth chunk, each
+// lane its dimensions, and the groups' sums meet in shared memory in a fixed order.
+template <int V>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
+    __shared__ float sw[256], red[16];
+    __shared__ float s_acc[8][32 * V];
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
+    const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
+    float m = -INFINITY, l = 0.0f;
+    if (tid < a.splits) {
+        l = a.part_l[base + tid];
+        if (l != 0.0f) m = a.part_m[base + tid];
+    }
+    float M = warp_max(m);
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+    M = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) M = fmaxf(M, red[i]);
+    const float e = l != 0.0f ? (m == -INFINITY ? 1.0f : exp2f(m - M)) : 0.0f;  // l without a maximum: NaN, as it is
+    sw[tid] = e;
+    float L = warp_sum(l * e);
+    if (lane == 0) red[8 + warp] = L;
+    __syncthreads();
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) L += red[8 + i];
+    if (a.stat && tid == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+    for (uint32_t d0 = 0; d0 < hd; d0 += 32u * V) {
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+        const uint32_t d = d0 + V * lane;
+        if (d < hd) {
+#pragma unroll 4
+            for (uint32_t s = warp; s < a.splits; s += 8u) {
+                const float w = sw[s];
+                const float* src = a.part_o + (base + s) * hd + d;
+                float x[V];
+                if (V == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(src);
+                    x[0] = y.x, x[V > 1 ? 1 : 0] = y.y, x[V > 2 ? 2 : 0] = y.z, x[V > 3 ? 3 : 0] = y.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[i] = src[i];
+                }
+                if (w != 0.0f)  // an empty part's outputs may be anything
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_acc[warp][i * 32 + lane] = acc[i];
+        __syncthreads();
+        if (warp == 0 && d < hd) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float o = s_acc[0][i * 32 + lane];
+#pragma unroll
+                for (int w = 1; w < 8; ++w) o += s_acc[w][i * 32 + lane];
+                a.out[head * hd + d + i] = L == 0.0f ? 0.0f : o / L;
+            }
+        }
+        __syncthreads();
+    }
 }
 
 // CTA = (256 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
@@ -286,6 +621,15 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a) {
         w += sum;
     }
     a.weights_out[at] = w;
+}
+
+template <int HD, bool WIDE>
+cudaError_t launch_tiles(const PagedAttnArgs& a, dim3 grid, uint32_t per, cudaStream_t s) {
+    constexpr size_t smem = (size_t)(HD == 128 ? 3 : 4) * 2 * TILE * HD * 2;
+    static_assert(smem >= (size_t)(WIDE ? 16 : 8) * (4 * 2 + 5 * HD + 2) * 4, "the parts lie over the ring");
+    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, grid, dim3(TILES_THREADS), smem, s, a, per);
 }
 
 template <typename ET, int GT>
@@ -358,7 +702,16 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     if (grid.y > 65535u) return M40LLM_ERR_LIMIT;
     const size_t smem = ((size_t)gt * hd4 + ROWS_THREADS * gt + gt * 32u + 8u + 64u) * 4u + 4ull * T * pitch * elem;
     cudaError_t e;
-    if (f32)
+    if (!f32 && vec && (hd == 64u || hd == 128u)) {
+        // heads of a group in equal shares of up to 16; 8 take one product where 9 to 16 take two
+        const uint32_t parts = (a.group + 15u) / 16u, per = (a.group + parts - 1) / parts;
+        const dim3 tiles(a.splits, cache->kv_heads * ((a.group + per - 1) / per), c->rows);
+        if (tiles.y > 65535u) return M40LLM_ERR_LIMIT;
+        if (hd == 64u)
+            e = per <= 8u ? launch_tiles<64, false>(a, tiles, per, s) : launch_tiles<64, true>(a, tiles, per, s);
+        else
+            e = per <= 8u ? launch_tiles<128, false>(a, tiles, per, s) : launch_tiles<128, true>(a, tiles, per, s);
+    } else if (f32)
         e = gt == 8   ? launch_rows<float, 8>(a, grid, T, vec, pitch, smem, s)
             : gt == 4 ? launch_rows<float, 4>(a, grid, T, vec, pitch, smem, s)
             : gt == 2 ? launch_rows<float, 2>(a, grid, T, vec, pitch, smem, s)
@@ -371,7 +724,8 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     M40_COUNT_LAUNCH(ctx);
     if (e != cudaSuccess) return cudaGetLastError(), -3;
     if (a.splits > 1 || a.scores) {
-        e = m40_launch_dependent(paged_merge_kernel, dim3(c->q_heads, c->rows), dim3(128), 0, s, a);
+        e = hd % 4u == 0 ? m40_launch_dependent(paged_merge_kernel<4>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a)
+                         : m40_launch_dependent(paged_merge_kernel<1>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a);
         M40_COUNT_LAUNCH(ctx);
     }
     if (e == cudaSuccess && a.scores) {
