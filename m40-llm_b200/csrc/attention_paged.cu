@@ -263,9 +263,16 @@ __device__ __noinline__ void paged_plain_head(const PagedAttnArgs& a, uint32_t s
 }
 
 // 16 bytes by cp.async; zeros where `bytes` is 0 (the source is then not read)
-__device__ __forceinline__ void cp_async16_or_zero(void* smem, const void* gmem, uint32_t bytes) {
-    const uint32_t s = (uint32_t)__cvta_generic_to_shared(smem);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(gmem), "r"(bytes));
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes));
+}
+__device__ __forceinline__ void ldmatrix_at(uint32_t (&r)[4], uint32_t smem) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t smem) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
 }
 
 constexpr uint32_t TILE = 64, TILES_THREADS = 128;
@@ -285,8 +292,6 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
     constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = HD == 128 ? 3 : 4, ROWS = WIDE ? 16 : 8;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t s_bad;
-    __half* sK = reinterpret_cast<__half*>(smem);
-    __half* sV = sK + STAGES * TILE * HD;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
     if (tid == 0) s_bad = 0u;
     pdl_wait();
@@ -310,28 +315,43 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
         return;
     }
     __syncthreads();
-    const uint32_t n_tiles = (t1 - t0 + TILE - 1) / TILE;
-    const __half* K = reinterpret_cast<const __half*>(a.c.k);
-    const __half* V = reinterpret_cast<const __half*>(a.c.v);
+    // tiles begin at multiples of 64, so that a tile is part of one page or whole pages
+    const uint32_t first = t0 & ~(TILE - 1u), n_tiles = (t1 - first + TILE - 1) / TILE;
+    constexpr uint32_t ROWS_AT_ONCE = TILES_THREADS / CHUNKS, COPIES = TILE / ROWS_AT_ONCE;  // a thread's rows lie a multiple of 8 apart: one swizzle for all
     const uint32_t* pages = a.c.table + (size_t)slot * a.c.max_pages;
-    const uint32_t in_page = (1u << a.c.shift) - 1u;
+    const uint32_t in_page = (1u << a.c.shift) - 1u, my_row = tid / CHUNKS, ch = tid % CHUNKS;
+    const uint32_t page_bytes = (a.c.kv_heads << a.c.shift) * (HD * 2u);
+    const unsigned char* srcK = a.c.k + ((size_t)kvh << a.c.shift) * (HD * 2u) + ch * 16u;
+    const ptrdiff_t toV = a.c.v - a.c.k;
+    const uint32_t ring = ((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u;  // whole rows, for the exclusive or below
+    const uint32_t toSV = STAGES * TILE * HD * 2u;
+    const uint32_t my_dst = ring + my_row * (HD * 2u) + ((ch ^ (my_row & 7u)) * 16u);
     auto load = [&](uint32_t tile) {
-        const uint32_t base = t0 + tile * TILE, stage = tile % STAGES, ch = tid % CHUNKS;
-        uint32_t page[TILE * CHUNKS / TILES_THREADS];
+        const uint32_t base = first + tile * TILE, dst = my_dst + (tile % STAGES) * (TILE * HD * 2u);
+        if (base >= t0 && base + TILE <= t1) {
+            const bool one = a.c.shift >= 6u;  // a tile within one page
+            uint32_t page[COPIES];
 #pragma unroll
-        for (int c = 0; c < (int)(TILE * CHUNKS / TILES_THREADS); ++c) {  // all lookups on their way together
-            const uint32_t e = base + c * (TILES_THREADS / CHUNKS) + tid / CHUNKS;
-            page[c] = e < t1 ? pages[e >> a.c.shift] : PAGED_NONE;
-        }
+            for (uint32_t c = 0; c < COPIES; ++c)  // all lookups on their way together
+                if (c == 0 || !one) page[c] = pages[(base + c * ROWS_AT_ONCE + my_row) >> a.c.shift];
 #pragma unroll
-        for (int c = 0; c < (int)(TILE * CHUNKS / TILES_THREADS); ++c) {
-            const uint32_t r = c * (TILES_THREADS / CHUNKS) + tid / CHUNKS, e = base + r;
-            const bool ok = page[c] < a.c.pages;
-            if (!ok && e < t1) s_bad = 1u;
-            const size_t src = ok ? ((((size_t)page[c] * a.c.kv_heads + kvh) << a.c.shift) + (e & in_page)) * HD + ch * 8u : 0;
-            const uint32_t dst = stage * TILE * HD + r * HD + ((ch ^ (r & 7u)) * 8u);
-            cp_async16_or_zero(sK + dst, K + src, ok ? 16u : 0u);
-            cp_async16_or_zero(sV + dst, V + src, ok ? 16u : 0u);
+            for (uint32_t c = 0; c < COPIES; ++c) {
+                const uint32_t pg = one ? page[0] : page[c], e = base + c * ROWS_AT_ONCE + my_row;
+                const bool ok = pg < a.c.pages;
+                if (!ok) s_bad = 1u;
+                const unsigned char* src = srcK + (ok ? (size_t)pg * page_bytes : 0) + (e & in_page) * (HD * 2u);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, src + toV, ok ? 16u : 0u);
+            }
+        } else {
+            for (uint32_t c = 0; c < COPIES; ++c) {
+                const uint32_t e = base + c * ROWS_AT_ONCE + my_row, pg = e >= t0 && e < t1 ? pages[e >> a.c.shift] : PAGED_NONE;
+                const bool ok = pg < a.c.pages;
+                if (!ok && e >= t0 && e < t1) s_bad = 1u;
+                const unsigned char* src = ok ? srcK + (size_t)pg * page_bytes + (e & in_page) * (HD * 2u) : a.c.k;
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, ok ? src + toV : a.c.v, ok ? 16u : 0u);
+            }
         }
     };
 #pragma unroll
@@ -371,47 +391,59 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
 #pragma unroll
     for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
 
+    // ldmatrix: the lane's row and 16-byte piece; the pieces of a product step follow by exclusive or
+    const uint32_t mj = lane >> 3, kr = warp * 16 + (mj >> 1) * 8 + (lane & 7u), vr = warp * 16 + (mj & 1u) * 8 + (lane & 7u);
+    const uint32_t k_at = ring + kr * (HD * 2u) + (((mj & 1u) ^ (kr & 7u)) * 16u);
+    const uint32_t v_at = ring + toSV + vr * (HD * 2u) + (((mj >> 1) ^ (vr & 7u)) * 16u);
     for (uint32_t tile = 0; tile < n_tiles; ++tile) {
         cp_async_wait<STAGES - 2>();
         __syncthreads();
         if (tile + STAGES - 1 < n_tiles) load(tile + STAGES - 1);
         cp_async_commit();
-        const __half* tK = sK + (size_t)(tile % STAGES) * TILE * HD;
-        const __half* tV = sV + (size_t)(tile % STAGES) * TILE * HD;
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-        {
-            const uint32_t j = lane >> 3, r = warp * 16 + (j >> 1) * 8 + (lane & 7u);
+        const uint32_t stage = (tile % STAGES) * (TILE * HD * 2u);
+        float s0[2][4], s1[2][4];  // even and odd product steps: two short chains each
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t ch = ks * 2 + (j & 1u);
-                uint32_t b[4];
-                ldmatrix_x4(b, tK + r * HD + ((ch ^ (r & 7u)) * 8));
-                mma16816(s0, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
-                mma16816(s1, qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
-                if (WIDE) {
-                    mma16816(s0, qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[0], b[1]);
-                    mma16816(s1, qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[2], b[3]);
-                }
+        for (int i = 0; i < 4; ++i) s0[0][i] = s0[1][i] = s1[0][i] = s1[1][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint32_t b[4];
+            ldmatrix_at(b, (k_at + stage) ^ (ks * 32u));
+            mma16816(s0[ks & 1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[0], b[1]);
+            mma16816(s1[ks & 1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b[2], b[3]);
+            if (WIDE) {
+                mma16816(s0[ks & 1], qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[0], b[1]);
+                mma16816(s1[ks & 1], qb[ks][0], qb[ks][1], qb[ks][2], qb[ks][3], b[2], b[3]);
             }
         }
         // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
-        const uint32_t e0 = t0 + tile * TILE + warp * 16 + 2 * t4;
+        const uint32_t base = first + tile * TILE, e0 = base + warp * 16 + 2 * t4;
         float s[H][4];
 #pragma unroll
+        for (int i = 0; i < 4; ++i) s0[0][i] += s0[1][i], s1[0][i] += s1[1][i];
+#pragma unroll
         for (int h = 0; h < H; ++h) {
-            s[h][0] = WIDE ? s0[2 * h] : s0[0] + s0[2], s[h][1] = WIDE ? s0[2 * h + 1] : s0[1] + s0[3];
-            s[h][2] = WIDE ? s1[2 * h] : s1[0] + s1[2], s[h][3] = WIDE ? s1[2 * h + 1] : s1[1] + s1[3];
+            s[h][0] = WIDE ? s0[0][2 * h] : s0[0][0] + s0[0][2], s[h][1] = WIDE ? s0[0][2 * h + 1] : s0[0][1] + s0[0][3];
+            s[h][2] = WIDE ? s1[0][2 * h] : s1[0][0] + s1[0][2], s[h][3] = WIDE ? s1[0][2 * h + 1] : s1[0][1] + s1[0][3];
         }
         const bool bad = *(volatile uint32_t*)&s_bad != 0u;
+        if (base < t0 || base + TILE > t1 || bad) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
-            const bool out = e >= t1 || (bad && pages[e >> a.c.shift] >= a.c.pages);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
+                if (e < t0 || e >= t1 || (bad && pages[e >> a.c.shift] >= a.c.pages)) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if (out) s[h][i] = -INFINITY;
-                if (a.scores && g + 8u * h < G && e < t1) a.scores[((size_t)row * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
+                    for (int h = 0; h < H; ++h) s[h][i] = -INFINITY;
+                }
             }
+        }
+        if (a.scores) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
+                    if (g + 8u * h < G && e >= t0 && e < t1) a.scores[((size_t)row * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
+                }
         }
         uint32_t ph[H][2], pl[H][2];
         bool moved = false;
@@ -438,22 +470,18 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
                 o[n][2] *= corr[H - 1], o[n][3] *= corr[H - 1];
             }
         }
-        {
-            const uint32_t j = lane >> 3, r = warp * 16 + (j & 1u) * 8 + (lane & 7u);
 #pragma unroll
-            for (int nd = 0; nd < HD / 16; ++nd) {
-                const uint32_t ch = nd * 2 + (j >> 1);
-                uint32_t b[4];
-                ldmatrix_x4_trans(b, tV + r * HD + ((ch ^ (r & 7u)) * 8));
-                if (WIDE) {
-                    mma16816(o[2 * nd], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[0], b[1]);
-                    mma16816(o[2 * nd + 1], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[2], b[3]);
-                    mma16816(o[2 * nd], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[0], b[1]);
-                    mma16816(o[2 * nd + 1], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[2], b[3]);
-                } else {
-                    mma16816(o[2 * nd], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[0], b[1]);
-                    mma16816(o[2 * nd + 1], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[2], b[3]);
-                }
+        for (int nd = 0; nd < HD / 16; ++nd) {
+            uint32_t b[4];
+            ldmatrix_trans_at(b, (v_at + stage) ^ (nd * 32u));
+            if (WIDE) {
+                mma16816(o[2 * nd], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[0], b[1]);
+                mma16816(o[2 * nd + 1], ph[0][0], ph[H - 1][0], ph[0][1], ph[H - 1][1], b[2], b[3]);
+                mma16816(o[2 * nd], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[0], b[1]);
+                mma16816(o[2 * nd + 1], pl[0][0], pl[H - 1][0], pl[0][1], pl[H - 1][1], b[2], b[3]);
+            } else {
+                mma16816(o[2 * nd], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[0], b[1]);
+                mma16816(o[2 * nd + 1], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[2], b[3]);
             }
         }
     }
@@ -625,7 +653,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a) {
 
 template <int HD, bool WIDE>
 cudaError_t launch_tiles(const PagedAttnArgs& a, dim3 grid, uint32_t per, cudaStream_t s) {
-    constexpr size_t smem = (size_t)(HD == 128 ? 3 : 4) * 2 * TILE * HD * 2;
+    constexpr size_t smem = (size_t)(HD == 128 ? 3 : 4) * 2 * TILE * HD * 2 + 256;
     static_assert(smem >= (size_t)(WIDE ? 16 : 8) * (4 * 2 + 5 * HD + 2) * 4, "the parts lie over the ring");
     const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
