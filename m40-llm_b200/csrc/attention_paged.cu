@@ -28,7 +28,9 @@ struct PagedAttnArgs {
     float* scores;  // [rows][q_heads][ld_scores] in base 2, or null
     float* stat;    // [rows][q_heads][2]: maximum, 1 / sum (0 for a row without entries), where scores are kept
     uint32_t* status;
+    uint64_t* prefix;  // paged_tiles_kernel: tiles before each row of the launch, [rows + 1]
     uint32_t rows, q_heads, group, splits, chunk, bound, ld_weights, ld_scores;
+    uint32_t row0, heads_at_once, ctas;  // paged_tiles_kernel: first row of the launch, q heads of one unit of work, resident CTAs
     float scale;  // times log2(e)
 };
 
@@ -39,9 +41,12 @@ __device__ __forceinline__ bool paged_row_range(const PagedAttnArgs& a, uint32_t
     *begin = a.row_begin ? a.row_begin[row] : 0u;
     return *slot < a.c.slots && *end <= a.bound;
 }
-// The part of them that split s covers; chunks are counted from the tile that `begin` lies in.
+// The part of them that split s covers: whole tiles of 64, counted from the one that `begin` lies in, dealt evenly to the splits, at least a.chunk
+// entries to each that has any.
 __device__ __forceinline__ void paged_chunk(const PagedAttnArgs& a, uint32_t split, uint32_t begin, uint32_t end, uint32_t* t0, uint32_t* t1) {
-    const uint64_t lo = (uint64_t)(begin & ~63u) + (uint64_t)split * a.chunk, hi = lo + a.chunk;
+    const uint32_t from = begin & ~63u, tiles = end > from ? (end - from + 63u) / 64u : 0u;
+    const uint32_t chunk = max((tiles + a.splits - 1u) / a.splits * 64u, a.chunk);
+    const uint64_t lo = (uint64_t)from + (uint64_t)split * chunk, hi = lo + chunk;
     *t0 = lo > begin ? (lo < end ? (uint32_t)lo : end) : begin;
     *t1 = hi < end ? (uint32_t)hi : end;
     if (*t1 < *t0) *t1 = *t0;
@@ -221,11 +226,12 @@ __global__ void __launch_bounds__(ROWS_THREADS) paged_rows_kernel(PagedAttnArgs 
         }
 }
 
-// One q head over the entries [t0, t1) of one kv head in plain f32, by one warp: what the matrix instructions cannot give where keys or values are
-// not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions 2 lane, 2 lane + 1 (+ 64). Scale as in PagedAttnArgs.
+// One q head over a warp's share of the entries [t0, t1) of one kv head (16 of every 64, from `share` on) in plain f32: what the matrix instructions
+// cannot give where keys or values are not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions
+// 2 lane, 2 lane + 1 (+ 64). Results as in paged_tiles_kernel.
 template <int HD>
-__device__ __noinline__ void paged_plain_head(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
-                                              uint32_t t1, float bias, float* m_out, float* l_out, float* o_out) {
+__device__ __noinline__ void paged_plain_share(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
+                                               uint32_t t1, uint32_t share, float bias, float* m_out, float* l_out, float* o_out) {
     const uint32_t lane = threadIdx.x & 31u, d = 2u * lane;
     const __half* K = reinterpret_cast<const __half*>(a.c.k);
     const __half* V = reinterpret_cast<const __half*>(a.c.v);
@@ -236,6 +242,7 @@ __device__ __noinline__ void paged_plain_head(const PagedAttnArgs& a, uint32_t s
         o[2 * j] = o[2 * j + 1] = 0.0f;
     }
     for (uint32_t e = t0; e < t1; ++e) {
+        if ((e & 63u) / 16u != share) continue;
         const uint32_t page = paged_page(a.c, slot, e);
         if (page == PAGED_NONE) continue;
         const size_t at = paged_row(a.c, page, kvh, e) + d;
@@ -259,7 +266,7 @@ __device__ __noinline__ void paged_plain_head(const PagedAttnArgs& a, uint32_t s
     }
     if (lane == 0) *m_out = m, *l_out = l;
 #pragma unroll
-    for (int j = 0; j < HD / 64; ++j) o_out[d + 64 * j] = o[2 * j], o_out[d + 64 * j + 1] = o[2 * j + 1];
+    for (int j = 0; j < HD / 64; ++j) *reinterpret_cast<float2*>(o_out + d + 64 * j) = make_float2(o[2 * j], o[2 * j + 1]);
 }
 
 // 16 bytes by cp.async; zeros where `bytes` is 0 (the source is then not read)
@@ -280,127 +287,218 @@ constexpr uint32_t TILE = 64, TILES_THREADS = 128;
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
 
-// CTA = (row, up to 8 (WIDE: 16) q heads of one kv head, chunk). K and V tiles of 64 entries come through a ring of cp.async stages, rows
-// looked up in the page table as they are fetched, into XOR-swizzled shared memory; a warp takes 16 entries of a tile.
+// The work of a launch is a list of tiles of 64 entries: rows in order, in a row the units of up to 8 (WIDE: 16) q heads of one kv head, in a unit
+// its tiles. Every resident CTA takes an equal run of the list, so that no CTA starts late and none ends early, whatever the lengths.
+// Each warp leaves its own (maximum, sum, output) of every unit that the run touches, without a barrier, and paged_join_kernel puts them together: the part
+// of CTA c in unit u of all units is number u + c, which no other has, as c or u grows from one part of the list to the next. Against one CTA per (row, unit, 1024 entries): 32 rows of up to 16384 entries 198 -> @A us,
+// one of 130001 110 -> @B.
+//   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units. A warp takes 16 entries.
 //   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them. A group has
 //                         at most 8 heads as a rule: hi and lo are then the two halves of the 16 rows of ONE operand, and the halves of the result are
 //                         added (WIDE: two products).
 //   softmax               online in base 2 per warp; the outputs are rescaled only when a maximum moved.
-// Two CTAs per SM with 96 (64) KB of ring each; bound by HBM for long chunks.
+constexpr uint32_t TILES_ROWS = 256;  // rows of a launch: their ranges stay in shared memory
+
+// The CTA whose run holds tile x of `total`; CTA i has [i total / n, (i + 1) total / n).
+__device__ __forceinline__ uint32_t cta_of(uint64_t x, uint64_t total, uint32_t n) { return (uint32_t)(((x + 1u) * n - 1u) / total); }
+__device__ __forceinline__ uint32_t ctas_at_work(uint64_t total, uint32_t n) { return total < n ? (uint32_t)total : n; }
+
 template <int HD, bool WIDE>
-__global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttnArgs a, uint32_t per) {
-    constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = HD == 128 ? 3 : 4, ROWS = WIDE ? 16 : 8;
+struct TilesCfg {
+    static constexpr int STAGES = HD == 128 ? 3 : 4, CTAS = HD == 128 ? 2 : 3;
+    static constexpr int RING = STAGES * 2 * (int)TILE * HD * 2;
+    static constexpr int SMEM = 256 + RING + (int)(TILES_ROWS + 1) * 8 + (int)TILES_ROWS * 12;  // ring, the prefix, the rows' ranges
+};
+
+template <int HD, bool WIDE>
+__global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) paged_tiles_kernel(PagedAttnArgs a) {
+    using Cfg = TilesCfg<HD, WIDE>;
+    constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = Cfg::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t s_bad;
+    const uint32_t ring = ((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u;  // whole rows, for the exclusive or below
+    uint64_t* s_prefix = reinterpret_cast<uint64_t*>(smem + 256 + Cfg::RING);
+    uint32_t* s_slot = reinterpret_cast<uint32_t*>(s_prefix + TILES_ROWS + 1);
+    uint32_t* s_begin = s_slot + TILES_ROWS;
+    uint32_t* s_end = s_begin + TILES_ROWS;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
+    const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = min(a.rows - a.row0, TILES_ROWS);
     if (tid == 0) s_bad = 0u;
     pdl_wait();
     pdl_trigger();
-    const uint32_t split = blockIdx.x, row = blockIdx.z, subgroups = (a.group + per - 1) / per;
-    const uint32_t kvh = blockIdx.y / subgroups, g0 = (blockIdx.y % subgroups) * per, G = min(per, a.group - g0), head0 = kvh * a.group + g0;
-    uint32_t slot, begin, end, t0 = 0, t1 = 0;
-    const bool inside = paged_row_range(a, row, &slot, &begin, &end);
-    if (!inside && tid == 0 && split == 0 && blockIdx.y == 0) atomicOr(a.status, 1u);
-    if (inside) paged_chunk(a, split, begin, end, &t0, &t1);
-    const bool partial = a.splits > 1 || a.scores;
-    if (t0 >= t1) {  // nothing in this chunk: an empty part (l = 0), or the row's zeros
-        for (uint32_t i = tid; i < G; i += TILES_THREADS)
-            if (partial) {
-                const size_t pi = ((size_t)row * a.q_heads + head0 + i) * a.splits + split;
-                a.part_m[pi] = -INFINITY;
-                a.part_l[pi] = 0.0f;
+    if (tid < 32u) {  // the rows' tiles, summed up by one warp
+        uint64_t before = 0;
+        for (uint32_t r0 = 0; r0 < rows; r0 += 32u) {
+            const uint32_t r = r0 + lane;
+            uint32_t slot = 0, begin = 0, end = 0, n = 0;
+            if (r < rows) {
+                const bool inside = paged_row_range(a, a.row0 + r, &slot, &begin, &end);
+                if (!inside && blockIdx.x == 0) atomicOr(a.status, 1u);
+                n = inside && end > begin ? (end - (begin & ~63u) + 63u) / 64u : 0u;
             }
-        if (!partial)
-            for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) a.out[((size_t)row * a.q_heads + head0) * HD + i] = 0.0f;
-        return;
+            uint64_t sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= (uint32_t)o) sum += u;
+            }
+            if (r < rows) {
+                s_slot[r] = slot, s_begin[r] = begin, s_end[r] = end;
+                s_prefix[r] = before + sum - n;
+                if (blockIdx.x == 0) a.prefix[r] = before + sum - n;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) {
+            s_prefix[rows] = before;
+            if (blockIdx.x == 0) a.prefix[rows] = before;
+        }
     }
     __syncthreads();
-    // tiles begin at multiples of 64, so that a tile is part of one page or whole pages
-    const uint32_t first = t0 & ~(TILE - 1u), n_tiles = (t1 - first + TILE - 1) / TILE;
+    const uint64_t total = s_prefix[rows] * units;
+    const uint32_t n_ctas = ctas_at_work(total, a.ctas);
+    if (blockIdx.x >= n_ctas) return;
+    const uint64_t lo = blockIdx.x * total / n_ctas;
+    const uint32_t count = (uint32_t)((blockIdx.x + 1u) * total / n_ctas - lo);  // at least 1
+
+    // a place in the list
+    struct Place {
+        uint32_t row, unit, tile, tiles, t0, t1, first;
+    };
+    auto enter = [&](Place& p) {  // p.row has tiles
+        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~63u;
+        p.tiles = (p.t1 - p.first + 63u) / 64u;
+    };
+    auto advance = [&](Place& p) {
+        if (++p.tile < p.tiles) return false;
+        p.tile = 0;
+        if (++p.unit == units) {
+            p.unit = 0;
+            do ++p.row;
+            while (p.row < rows && s_prefix[p.row + 1] == s_prefix[p.row]);
+            if (p.row < rows) enter(p);
+        }
+        return true;
+    };
+    Place at;
+    {
+        uint32_t l = 0, h = rows;  // the last row that begins at or before lo
+        while (h - l > 1u) {
+            const uint32_t mid = (l + h) / 2u;
+            if (s_prefix[mid] * units <= lo) l = mid; else h = mid;
+        }
+        at.row = l;
+        enter(at);
+        const uint64_t in_row = lo - s_prefix[l] * units;
+        at.unit = (uint32_t)(in_row / at.tiles);
+        at.tile = (uint32_t)(in_row - (uint64_t)at.unit * at.tiles);
+    }
+
     constexpr uint32_t ROWS_AT_ONCE = TILES_THREADS / CHUNKS, COPIES = TILE / ROWS_AT_ONCE;  // a thread's rows lie a multiple of 8 apart: one swizzle for all
-    const uint32_t* pages = a.c.table + (size_t)slot * a.c.max_pages;
+    const uint32_t subgroups = units / a.c.kv_heads;
     const uint32_t in_page = (1u << a.c.shift) - 1u, my_row = tid / CHUNKS, ch = tid % CHUNKS;
-    const uint32_t page_bytes = (a.c.kv_heads << a.c.shift) * (HD * 2u);
-    const unsigned char* srcK = a.c.k + ((size_t)kvh << a.c.shift) * (HD * 2u) + ch * 16u;
+    const uint64_t head_bytes = (uint64_t)(HD * 2u) << a.c.shift;
+    const uint64_t page_bytes = a.c.kv_heads * head_bytes;
     const ptrdiff_t toV = a.c.v - a.c.k;
-    const uint32_t ring = ((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u;  // whole rows, for the exclusive or below
     const uint32_t toSV = STAGES * TILE * HD * 2u;
     const uint32_t my_dst = ring + my_row * (HD * 2u) + ((ch ^ (my_row & 7u)) * 16u);
-    auto load = [&](uint32_t tile) {
-        const uint32_t base = first + tile * TILE, dst = my_dst + (tile % STAGES) * (TILE * HD * 2u);
-        if (base >= t0 && base + TILE <= t1) {
-            const bool one = a.c.shift >= 6u;  // a tile within one page
-            uint32_t page[COPIES];
-#pragma unroll
-            for (uint32_t c = 0; c < COPIES; ++c)  // all lookups on their way together
-                if (c == 0 || !one) page[c] = pages[(base + c * ROWS_AT_ONCE + my_row) >> a.c.shift];
-#pragma unroll
+    Place fetch = at;
+    const uint32_t* pages = nullptr;
+    const unsigned char* srcK = nullptr;
+    auto aim = [&]() {
+        pages = a.c.table + (size_t)s_slot[fetch.row] * a.c.max_pages;
+        srcK = a.c.k + fetch.unit / subgroups * head_bytes + ch * 16u;
+    };
+    auto load = [&](uint32_t f) {  // tile f of the run, where `fetch` is
+        const uint32_t base = fetch.first + fetch.tile * TILE, dst = my_dst + (f % STAGES) * (TILE * HD * 2u);
+        if (base < fetch.t0 || base + TILE > fetch.t1) {
             for (uint32_t c = 0; c < COPIES; ++c) {
-                const uint32_t pg = one ? page[0] : page[c], e = base + c * ROWS_AT_ONCE + my_row;
+                const uint32_t e = base + c * ROWS_AT_ONCE + my_row, pg = e >= fetch.t0 && e < fetch.t1 ? pages[e >> a.c.shift] : PAGED_NONE;
                 const bool ok = pg < a.c.pages;
-                if (!ok) s_bad = 1u;
-                const unsigned char* src = srcK + (ok ? (size_t)pg * page_bytes : 0) + (e & in_page) * (HD * 2u);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, src + toV, ok ? 16u : 0u);
-            }
-        } else {
-            for (uint32_t c = 0; c < COPIES; ++c) {
-                const uint32_t e = base + c * ROWS_AT_ONCE + my_row, pg = e >= t0 && e < t1 ? pages[e >> a.c.shift] : PAGED_NONE;
-                const bool ok = pg < a.c.pages;
-                if (!ok && e >= t0 && e < t1) s_bad = 1u;
-                const unsigned char* src = ok ? srcK + (size_t)pg * page_bytes + (e & in_page) * (HD * 2u) : a.c.k;
+                if (!ok && e >= fetch.t0 && e < fetch.t1) s_bad = 1u;
+                const unsigned char* src = ok ? srcK + pg * page_bytes + (e & in_page) * (HD * 2u) : a.c.k;
                 cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
                 cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, ok ? src + toV : a.c.v, ok ? 16u : 0u);
             }
+        } else if (a.c.shift >= 6u) {  // a tile within one page
+            const uint32_t pg = pages[base >> a.c.shift];
+            const bool ok = pg < a.c.pages;
+            if (!ok) s_bad = 1u;
+            const unsigned char* src = srcK + (ok ? pg * page_bytes : 0) + ((base & in_page) + my_row) * (HD * 2u);
+            const unsigned char* srcV = src + toV;
+            const uint32_t bytes = ok ? 16u : 0u;
+#pragma unroll
+            for (uint32_t c = 0; c < COPIES; ++c) {
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src + c * (ROWS_AT_ONCE * HD * 2u), bytes);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, srcV + c * (ROWS_AT_ONCE * HD * 2u), bytes);
+            }
+        } else {
+            uint32_t page[COPIES];
+#pragma unroll
+            for (uint32_t c = 0; c < COPIES; ++c) page[c] = pages[(base + c * ROWS_AT_ONCE + my_row) >> a.c.shift];  // all lookups on their way together
+#pragma unroll
+            for (uint32_t c = 0; c < COPIES; ++c) {
+                const uint32_t e = base + c * ROWS_AT_ONCE + my_row;
+                const bool ok = page[c] < a.c.pages;
+                if (!ok) s_bad = 1u;
+                const unsigned char* src = srcK + (ok ? page[c] * page_bytes : 0) + (e & in_page) * (HD * 2u);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
+                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, src + toV, ok ? 16u : 0u);
+            }
         }
+        if (advance(fetch) && f + 1u < count) aim();
     };
+    aim();
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-        if ((uint32_t)s < n_tiles) load(s);
+        if ((uint32_t)s < count) load(s);
         cp_async_commit();
     }
-
-    // A operand of the scores: rows 0-7 hi, 8-15 lo of heads 0-7; WIDE: rows are heads, hi and lo apart
-    uint32_t qa[KS][4], qb[WIDE ? KS : 1][4];
-    {
-        const float* q0 = a.q + ((size_t)row * a.q_heads + head0 + g) * HD;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t k0 = ks * 16 + half * 8 + 2 * t4;
-                const float x = g < G ? q0[k0] * a.scale : 0.0f, y = g < G ? q0[k0 + 1] * a.scale : 0.0f;
-                uint32_t hi, lo;
-                split_h2(x, y, &hi, &lo);
-                qa[ks][2 * half] = hi;
-                if (WIDE) {
-                    qb[ks][2 * half] = lo;
-                    const float* q1 = q0 + 8 * HD;
-                    const float u = g + 8u < G ? q1[k0] * a.scale : 0.0f, w = g + 8u < G ? q1[k0 + 1] * a.scale : 0.0f;
-                    split_h2(u, w, &qa[ks][2 * half + 1], &qb[ks][2 * half + 1]);
-                } else {
-                    qa[ks][2 * half + 1] = lo;
-                }
-            }
-    }
-    float o[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    constexpr int H = WIDE ? 2 : 1;  // heads of a thread
-    float m_run[H], l_run[H];
-#pragma unroll
-    for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
 
     // ldmatrix: the lane's row and 16-byte piece; the pieces of a product step follow by exclusive or
     const uint32_t mj = lane >> 3, kr = warp * 16 + (mj >> 1) * 8 + (lane & 7u), vr = warp * 16 + (mj & 1u) * 8 + (lane & 7u);
     const uint32_t k_at = ring + kr * (HD * 2u) + (((mj & 1u) ^ (kr & 7u)) * 16u);
     const uint32_t v_at = ring + toSV + vr * (HD * 2u) + (((mj >> 1) ^ (vr & 7u)) * 16u);
-    for (uint32_t tile = 0; tile < n_tiles; ++tile) {
+    constexpr int H = WIDE ? 2 : 1;  // heads of a thread
+    uint32_t qa[KS][4], qb[WIDE ? KS : 1][4];
+    float o[NT][4], m_run[H], l_run[H];
+    uint32_t head0 = 0, G = 0, tile_begin = 0;
+    bool entering = true;
+    for (uint32_t f = 0; f < count; ++f) {
+        if (entering) {
+            const uint32_t kvh = at.unit / subgroups, g0 = (at.unit - kvh * subgroups) * a.heads_at_once;
+            G = min(a.heads_at_once, a.group - g0);
+            head0 = kvh * a.group + g0;
+            tile_begin = at.tile;
+            // A operand of the scores: rows 0-7 hi, 8-15 lo of heads 0-7; WIDE: rows are heads, hi and lo apart
+            const float* q0 = a.q + ((size_t)(a.row0 + at.row) * a.q_heads + head0 + g) * HD;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t k0 = ks * 16 + half * 8 + 2 * t4;
+                    const float2 x = g < G ? *reinterpret_cast<const float2*>(q0 + k0) : make_float2(0.0f, 0.0f);
+                    uint32_t hi, lo_part;
+                    split_h2(x.x * a.scale, x.y * a.scale, &hi, &lo_part);
+                    qa[ks][2 * half] = hi;
+                    if (WIDE) {
+                        qb[ks][2 * half] = lo_part;
+                        const float2 y = g + 8u < G ? *reinterpret_cast<const float2*>(q0 + 8 * HD + k0) : make_float2(0.0f, 0.0f);
+                        split_h2(y.x * a.scale, y.y * a.scale, &qa[ks][2 * half + 1], &qb[ks][2 * half + 1]);
+                    } else {
+                        qa[ks][2 * half + 1] = lo_part;
+                    }
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
+        }
         cp_async_wait<STAGES - 2>();
         __syncthreads();
-        if (tile + STAGES - 1 < n_tiles) load(tile + STAGES - 1);
+        if (f + STAGES - 1 < count) load(f + STAGES - 1);
         cp_async_commit();
-        const uint32_t stage = (tile % STAGES) * (TILE * HD * 2u);
+        const uint32_t stage = (f % STAGES) * (TILE * HD * 2u);
         float s0[2][4], s1[2][4];  // even and odd product steps: two short chains each
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] = s0[1][i] = s1[0][i] = s1[1][i] = 0.0f;
@@ -416,7 +514,7 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
             }
         }
         // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
-        const uint32_t base = first + tile * TILE, e0 = base + warp * 16 + 2 * t4;
+        const uint32_t base = at.first + at.tile * TILE, e0 = base + warp * 16 + 2 * t4;
         float s[H][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] += s0[1][i], s1[0][i] += s1[1][i];
@@ -426,11 +524,12 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
             s[h][2] = WIDE ? s1[0][2 * h] : s1[0][0] + s1[0][2], s[h][3] = WIDE ? s1[0][2 * h + 1] : s1[0][1] + s1[0][3];
         }
         const bool bad = *(volatile uint32_t*)&s_bad != 0u;
-        if (base < t0 || base + TILE > t1 || bad) {
+        if (base < at.t0 || base + TILE > at.t1 || bad) {
+            const uint32_t* own_pages = a.c.table + (size_t)s_slot[at.row] * a.c.max_pages;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
-                if (e < t0 || e >= t1 || (bad && pages[e >> a.c.shift] >= a.c.pages)) {
+                if (e < at.t0 || e >= at.t1 || (bad && own_pages[e >> a.c.shift] >= a.c.pages)) {
 #pragma unroll
                     for (int h = 0; h < H; ++h) s[h][i] = -INFINITY;
                 }
@@ -442,7 +541,8 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
-                    if (g + 8u * h < G && e >= t0 && e < t1) a.scores[((size_t)row * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
+                    if (g + 8u * h < G && e >= at.t0 && e < at.t1)
+                        a.scores[((size_t)(a.row0 + at.row) * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
                 }
         }
         uint32_t ph[H][2], pl[H][2];
@@ -484,95 +584,85 @@ __global__ void __launch_bounds__(TILES_THREADS, 2) paged_tiles_kernel(PagedAttn
                 mma16816(o[2 * nd + 1], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[2], b[3]);
             }
         }
+
+        const bool ends = at.tile + 1u == at.tiles;
+        if (ends || f + 1u == count) {
+            // this warp's part of the unit
+            const uint32_t row = a.row0 + at.row, kvh = at.unit / subgroups;
+            const size_t part = (((size_t)at.row * units + at.unit + blockIdx.x) * 4u + warp) * a.heads_at_once;
+            bool fine[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                float l = l_run[h];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                fine[h] = is_finite(l);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if (!WIDE) o[n][0] += o[n][2], o[n][1] += o[n][3];
+                    fine[h] &= is_finite(o[n][2 * h]) & is_finite(o[n][2 * h + 1]);
+                }
+                if (g + 8u * h < G) {
+                    if (t4 == 0) a.part_m[part + g + 8 * h] = m_run[h], a.part_l[part + g + 8 * h] = l;
+                    float* dst = a.part_o + (part + g + 8 * h) * HD + 2 * t4;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                uint32_t odd = __ballot_sync(0xffffffffu, !fine[h] && g + 8u * h < G);
+                while (odd) {  // a head with something that is not finite: again, in plain f32
+                    const uint32_t gh = (__ffs(odd) - 1u) / 4u, head = head0 + gh + 8u * h;
+                    odd &= ~(0xfu << (4u * gh));
+                    const size_t at_part = part + gh + 8u * h, at_head = (size_t)row * a.q_heads + head;
+                    __syncwarp();
+                    paged_plain_share<HD>(a, s_slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
+                                          max(at.t0, at.first + tile_begin * TILE), min(at.t1, base + TILE), warp, WEIGHT_BIAS, a.part_m + at_part,
+                                          a.part_l + at_part, a.part_o + at_part * HD);
+                }
+            }
+        }
+        entering = advance(at);
     }
     cp_async_wait<0>();
-    __syncthreads();
-
-    // the four warps' parts through shared memory, over the ring that is done with
-    float* sm_m = reinterpret_cast<float*>(smem);  // [4][ROWS]
-    float* sm_l = sm_m + 4 * ROWS;                 // [4][ROWS]
-    float* sm_o = sm_l + 4 * ROWS;                 // [4][ROWS][HD], then the heads' own [ROWS][HD]
-    float* sm_r = sm_o + 4 * ROWS * HD;
-    float* sm_t = sm_r + ROWS * HD;                // [ROWS][2]: m, l of the heads
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-        float l = l_run[h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t4 == 0) sm_m[warp * ROWS + g + 8 * h] = m_run[h], sm_l[warp * ROWS + g + 8 * h] = l;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        float* dst = sm_o + ((size_t)warp * ROWS + g) * HD + n * 8 + 2 * t4;
-        if (WIDE) {
-            dst[0] = o[n][0], dst[1] = o[n][1];
-            dst[8 * HD] = o[n][2], dst[8 * HD + 1] = o[n][3];
-        } else {
-            dst[0] = o[n][0] + o[n][2], dst[1] = o[n][1] + o[n][3];
-        }
-    }
-    __syncthreads();
     if (s_bad && tid == 0) atomicOr(a.status, 1u);
-    // a warp finishes a head at a time
-    for (uint32_t h = warp; h < G; h += 4u) {
-        float M = -INFINITY, L = 0.0f, e[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w * ROWS + h]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float mw = sm_m[w * ROWS + h], lw = sm_l[w * ROWS + h];
-            e[w] = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : exp2f(mw - M);
-            L += lw * e[w];
-        }
-        bool fine = is_finite(L);
-        for (uint32_t d = lane; d < HD; d += 32u) {
-            float O = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) O += sm_o[((size_t)w * ROWS + h) * HD + d] * e[w];
-            sm_r[h * HD + d] = O;
-            fine &= is_finite(O);
-        }
-        const size_t head = (size_t)row * a.q_heads + head0 + h;
-        if (!__all_sync(0xffffffffu, fine)) {
-            paged_plain_head<HD>(a, slot, kvh, a.q + head * HD, a.scores ? a.scores + head * a.ld_scores : nullptr, t0, t1, WEIGHT_BIAS, sm_t + 2 * h,
-                                 sm_t + 2 * h + 1, sm_r + h * HD);
-            __syncwarp();
-            M = sm_t[2 * h], L = sm_t[2 * h + 1];
-        }
-        __syncwarp();
-        if (partial) {
-            if (lane == 0) a.part_m[head * a.splits + split] = M, a.part_l[head * a.splits + split] = L;
-            for (uint32_t d = lane; d < HD; d += 32u) a.part_o[(head * a.splits + split) * HD + d] = sm_r[h * HD + d];
-        } else {
-            for (uint32_t d = lane; d < HD; d += 32u) a.out[head * HD + d] = L == 0.0f ? 0.0f : sm_r[h * HD + d] / L;
-        }
-    }
 }
 
-// CTA = (q head, row): the chunks' parts in order. Thread s has chunk s's weight (at most 256 chunks); then eight groups of lanes take every eighth chunk, each
-// lane its dimensions, and the groups' sums meet in shared memory in a fixed order.
-template <int V>
-__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
-    __shared__ float sw[256], red[16];
+// The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most 1792: four warps of 444 CTAs); then eight groups of lanes take every
+// eighth part, each lane its dimensions, and the groups' sums meet in shared memory.
+template <int V, typename Part>
+__device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t parts, Part part) {
+    constexpr uint32_t MOST = 1792;
+    __shared__ float sw[MOST], red[16];
     __shared__ float s_acc[8][32 * V];
-    pdl_wait();
-    pdl_trigger();
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
-    const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
-    float m = -INFINITY, l = 0.0f;
-    if (tid < a.splits) {
-        l = a.part_l[base + tid];
-        if (l != 0.0f) m = a.part_m[base + tid];
+    float m[MOST / 256], l[MOST / 256], M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < MOST / 256u; ++j) {
+        const uint32_t s = tid + 256u * j;
+        m[j] = -INFINITY, l[j] = 0.0f;
+        if (256u * j >= parts) continue;
+        if (s < parts) {
+            l[j] = a.part_l[part(s)];
+            if (l[j] != 0.0f) m[j] = a.part_m[part(s)];
+        }
+        M = fmaxf(M, m[j]);
     }
-    float M = warp_max(m);
+    M = warp_max(M);
     if (lane == 0) red[warp] = M;
     __syncthreads();
     M = red[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) M = fmaxf(M, red[i]);
-    const float e = l != 0.0f ? (m == -INFINITY ? 1.0f : exp2f(m - M)) : 0.0f;  // l without a maximum: NaN, as it is
-    sw[tid] = e;
-    float L = warp_sum(l * e);
+#pragma unroll
+    for (uint32_t j = 0; j < MOST / 256u; ++j) {
+        if (256u * j >= parts) continue;
+        const float e = l[j] != 0.0f ? (m[j] == -INFINITY ? 1.0f : exp2f(m[j] - M)) : 0.0f;  // a sum without a maximum: NaN, as it is
+        sw[tid + 256u * j] = e;
+        L += l[j] * e;
+    }
+    L = warp_sum(L);
     if (lane == 0) red[8 + warp] = L;
     __syncthreads();
     L = 0.0f;
@@ -586,13 +676,13 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
         const uint32_t d = d0 + V * lane;
         if (d < hd) {
 #pragma unroll 4
-            for (uint32_t s = warp; s < a.splits; s += 8u) {
+            for (uint32_t s = warp; s < parts; s += 8u) {
                 const float w = sw[s];
-                const float* src = a.part_o + (base + s) * hd + d;
+                const float* src = a.part_o + part(s) * hd + d;
                 float x[V];
-                if (V == 4) {
+                if constexpr (V == 4) {
                     const float4 y = *reinterpret_cast<const float4*>(src);
-                    x[0] = y.x, x[V > 1 ? 1 : 0] = y.y, x[V > 2 ? 2 : 0] = y.z, x[V > 3 ? 3 : 0] = y.w;
+                    x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
                 } else {
 #pragma unroll
                     for (int i = 0; i < V; ++i) x[i] = src[i];
@@ -616,6 +706,35 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
         }
         __syncthreads();
     }
+}
+
+// Parts of paged_rows_kernel: [row][q head][split].
+template <int V>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
+    paged_join_parts<V>(a, head, a.splits, [=](uint32_t s) { return base + s; });
+}
+
+// Parts of paged_tiles_kernel, and the zeros of rows without entries. Grid (q head, row of the launch).
+__global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t r = blockIdx.y, rows = gridDim.y, kvh = blockIdx.x / a.group, in_group = blockIdx.x - kvh * a.group;
+    const uint32_t subgroups = (a.group + a.heads_at_once - 1u) / a.heads_at_once, units = a.c.kv_heads * subgroups;
+    const uint32_t unit = kvh * subgroups + in_group / a.heads_at_once, h = in_group % a.heads_at_once;
+    const size_t head = (size_t)(a.row0 + r) * a.q_heads + blockIdx.x;
+    const uint64_t before = a.prefix[r], tiles = a.prefix[r + 1] - before, total = a.prefix[rows] * units;
+    if (tiles == 0) {
+        for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
+        return;
+    }
+    const uint32_t n = ctas_at_work(total, a.ctas);
+    const uint64_t lo = before * units + unit * tiles;
+    const uint32_t c0 = cta_of(lo, total, n), c1 = cta_of(lo + tiles - 1u, total, n);
+    const size_t part = ((size_t)r * units + unit + c0) * 4u;  // four warps' parts for every CTA
+    paged_join_parts<4>(a, head, 4u * (c1 - c0 + 1u), [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
 }
 
 // CTA = (256 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
@@ -651,13 +770,20 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a) {
     a.weights_out[at] = w;
 }
 
+// All rows in launches of up to 256, each followed by its join.
 template <int HD, bool WIDE>
-cudaError_t launch_tiles(const PagedAttnArgs& a, dim3 grid, uint32_t per, cudaStream_t s) {
-    constexpr size_t smem = (size_t)(HD == 128 ? 3 : 4) * 2 * TILE * HD * 2 + 256;
-    static_assert(smem >= (size_t)(WIDE ? 16 : 8) * (4 * 2 + 5 * HD + 2) * 4, "the parts lie over the ring");
-    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, grid, dim3(TILES_THREADS), smem, s, a, per);
+cudaError_t launch_tiles(M40llmCudaContext* ctx, PagedAttnArgs a) {
+    using Cfg = TilesCfg<HD, WIDE>;
+    cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    a.ctas = (uint32_t)ctx->sm_count * Cfg::CTAS;
+    for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += TILES_ROWS) {
+        const uint32_t rows = a.rows - a.row0 < TILES_ROWS ? a.rows - a.row0 : TILES_ROWS;
+        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.ctas), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
+        if (e == cudaSuccess) e = m40_launch_dependent(paged_join_kernel, dim3(a.q_heads, rows), dim3(256), 0, ctx->decode_stream, a);
+        M40_COUNT_LAUNCH(ctx);
+        M40_COUNT_LAUNCH(ctx);
+    }
+    return e;
 }
 
 template <typename ET, int GT>
@@ -698,21 +824,34 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     a.ld_weights = c->ld_weights;
     a.bound = c->max_len ? c->max_len : capacity;
     a.scale = c->scale * LOG2E;
-    const uint32_t covered = a.bound;
-    const uint64_t work = (uint64_t)c->rows * cache->kv_heads * covered, target = 2ull * (uint64_t)ctx->sm_count;
-    uint64_t chunk = (work + target - 1) / target;
-    chunk = chunk < 128u ? 128u : (chunk > 1024u ? 1024u : chunk);
-    chunk = (chunk + 63u) & ~63ull;
-    if ((covered + chunk - 1) / chunk > 256u) chunk = ((covered + 255u) / 256u + 63u) & ~63ull;
-    a.chunk = (uint32_t)chunk;
-    a.splits = (uint32_t)((covered + chunk - 1) / chunk);
+    cudaStream_t s = ctx->decode_stream;
+    const bool f32 = cache->elem_dtype == M40LLM_DT_F32;
+    const uint32_t vec = m40_paged_vec16(cache) ? 1u : 0u;
+    const bool tiles = !f32 && vec && (hd == 64u || hd == 128u) && (((uintptr_t)c->q) & 7u) == 0;
+    // heads of a group in equal shares of up to 16; 8 take one product where 9 to 16 take two
+    const uint32_t shares = (a.group + 15u) / 16u;
+    a.heads_at_once = (a.group + shares - 1) / shares;
+    if (!tiles) {
+        const uint64_t work = (uint64_t)c->rows * cache->kv_heads * a.bound, target = 2ull * (uint64_t)ctx->sm_count;
+        uint64_t chunk = (work + target - 1) / target;
+        chunk = chunk < 128u ? 128u : (chunk > 1024u ? 1024u : chunk);
+        chunk = (chunk + 63u) & ~63ull;
+        if ((a.bound + chunk - 1) / chunk > 256u) chunk = ((a.bound + 255u) / 256u + 63u) & ~63ull;
+        a.chunk = (uint32_t)chunk;
+        a.splits = (uint32_t)((a.bound + chunk - 1) / chunk);
+    }
     const size_t heads = (size_t)c->rows * c->q_heads;
-    if (a.splits > 1 || c->weights_out) {
+    if (tiles || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? a.bound : 0u;
-        const size_t parts = heads * a.splits, floats = parts * (hd + 2) + heads * 2 + heads * (size_t)a.ld_scores;
-        float* work_area = (float*)m40_ensure_scratch(ctx, 1, floats * sizeof(float), 0);
+        const size_t rows_at_once = c->rows < TILES_ROWS ? c->rows : TILES_ROWS;
+        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u)) * 4u * a.heads_at_once
+                                   : heads * a.splits;
+        const size_t floats = parts * (hd + 2) + heads * 2 + heads * (size_t)a.ld_scores;
+        const size_t prefix = (TILES_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
+        unsigned char* work_area = (unsigned char*)m40_ensure_scratch(ctx, 1, prefix + 8 + floats * sizeof(float), 0);
         if (!work_area) return -5;
-        a.part_o = work_area;
+        a.prefix = (uint64_t*)work_area;
+        a.part_o = (float*)(work_area + prefix + 8);
         a.part_m = a.part_o + parts * hd;
         a.part_l = a.part_m + parts;
         if (c->weights_out) {
@@ -720,45 +859,43 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
             a.scores = a.stat + 2 * heads;
         }
     }
-    cudaStream_t s = ctx->decode_stream;
-    const bool f32 = cache->elem_dtype == M40LLM_DT_F32;
-    const uint32_t elem = f32 ? 4u : 2u, hd4 = (hd + 3u) & ~3u;
-    const uint32_t T = hd4 * elem > 1024u ? 16u : 32u, pitch = ((hd4 * elem + 15u) & ~15u) / elem + 16u / elem;
-    const uint32_t vec = m40_paged_vec16(cache) ? 1u : 0u;
-    const uint32_t gt = a.group >= 8u ? 8u : (a.group >= 4u ? 4u : (a.group >= 2u ? 2u : 1u)), subgroups = (a.group + gt - 1) / gt;
-    const dim3 grid(a.splits, cache->kv_heads * subgroups, c->rows);
-    if (grid.y > 65535u) return M40LLM_ERR_LIMIT;
-    const size_t smem = ((size_t)gt * hd4 + ROWS_THREADS * gt + gt * 32u + 8u + 64u) * 4u + 4ull * T * pitch * elem;
     cudaError_t e;
-    if (!f32 && vec && (hd == 64u || hd == 128u)) {
-        // heads of a group in equal shares of up to 16; 8 take one product where 9 to 16 take two
-        const uint32_t parts = (a.group + 15u) / 16u, per = (a.group + parts - 1) / parts;
-        const dim3 tiles(a.splits, cache->kv_heads * ((a.group + per - 1) / per), c->rows);
-        if (tiles.y > 65535u) return M40LLM_ERR_LIMIT;
+    if (tiles) {
         if (hd == 64u)
-            e = per <= 8u ? launch_tiles<64, false>(a, tiles, per, s) : launch_tiles<64, true>(a, tiles, per, s);
+            e = a.heads_at_once <= 8u ? launch_tiles<64, false>(ctx, a) : launch_tiles<64, true>(ctx, a);
         else
-            e = per <= 8u ? launch_tiles<128, false>(a, tiles, per, s) : launch_tiles<128, true>(a, tiles, per, s);
-    } else if (f32)
-        e = gt == 8   ? launch_rows<float, 8>(a, grid, T, vec, pitch, smem, s)
-            : gt == 4 ? launch_rows<float, 4>(a, grid, T, vec, pitch, smem, s)
-            : gt == 2 ? launch_rows<float, 2>(a, grid, T, vec, pitch, smem, s)
-                      : launch_rows<float, 1>(a, grid, T, vec, pitch, smem, s);
-    else
-        e = gt == 8   ? launch_rows<__half, 8>(a, grid, T, vec, pitch, smem, s)
-            : gt == 4 ? launch_rows<__half, 4>(a, grid, T, vec, pitch, smem, s)
-            : gt == 2 ? launch_rows<__half, 2>(a, grid, T, vec, pitch, smem, s)
-                      : launch_rows<__half, 1>(a, grid, T, vec, pitch, smem, s);
-    M40_COUNT_LAUNCH(ctx);
-    if (e != cudaSuccess) return cudaGetLastError(), -3;
-    if (a.splits > 1 || a.scores) {
-        e = hd % 4u == 0 ? m40_launch_dependent(paged_merge_kernel<4>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a)
-                         : m40_launch_dependent(paged_merge_kernel<1>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a);
+            e = a.heads_at_once <= 8u ? launch_tiles<128, false>(ctx, a) : launch_tiles<128, true>(ctx, a);
+    } else {
+        const uint32_t elem = f32 ? 4u : 2u, hd4 = (hd + 3u) & ~3u;
+        const uint32_t T = hd4 * elem > 1024u ? 16u : 32u, pitch = ((hd4 * elem + 15u) & ~15u) / elem + 16u / elem;
+        const uint32_t gt = a.group >= 8u ? 8u : (a.group >= 4u ? 4u : (a.group >= 2u ? 2u : 1u)), subgroups = (a.group + gt - 1) / gt;
+        const dim3 grid(a.splits, cache->kv_heads * subgroups, c->rows);
+        if (grid.y > 65535u) return M40LLM_ERR_LIMIT;
+        const size_t smem = ((size_t)gt * hd4 + ROWS_THREADS * gt + gt * 32u + 8u + 64u) * 4u + 4ull * T * pitch * elem;
+        if (f32)
+            e = gt == 8   ? launch_rows<float, 8>(a, grid, T, vec, pitch, smem, s)
+                : gt == 4 ? launch_rows<float, 4>(a, grid, T, vec, pitch, smem, s)
+                : gt == 2 ? launch_rows<float, 2>(a, grid, T, vec, pitch, smem, s)
+                          : launch_rows<float, 1>(a, grid, T, vec, pitch, smem, s);
+        else
+            e = gt == 8   ? launch_rows<__half, 8>(a, grid, T, vec, pitch, smem, s)
+                : gt == 4 ? launch_rows<__half, 4>(a, grid, T, vec, pitch, smem, s)
+                : gt == 2 ? launch_rows<__half, 2>(a, grid, T, vec, pitch, smem, s)
+                          : launch_rows<__half, 1>(a, grid, T, vec, pitch, smem, s);
         M40_COUNT_LAUNCH(ctx);
+        if (e == cudaSuccess && (a.splits > 1 || a.scores)) {
+            e = hd % 4u == 0 ? m40_launch_dependent(paged_merge_kernel<4>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a)
+                             : m40_launch_dependent(paged_merge_kernel<1>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a);
+            M40_COUNT_LAUNCH(ctx);
+        }
     }
     if (e == cudaSuccess && a.scores) {
         e = m40_launch_dependent(paged_weights_kernel, dim3((a.bound + 255u) / 256u, cache->kv_heads, c->rows), dim3(256), 0, s, a);
         M40_COUNT_LAUNCH(ctx);
     }
-    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -3;
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return -3;
+    }
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
