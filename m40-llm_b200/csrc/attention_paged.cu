@@ -30,7 +30,7 @@ struct PagedAttnArgs {
     uint32_t* status;
     uint64_t* prefix;  // paged_tiles_kernel: tiles before each row of the launch, [rows + 1]
     uint32_t rows, q_heads, group, splits, chunk, bound, ld_weights, ld_scores;
-    uint32_t row0, heads_at_once, ctas;  // paged_tiles_kernel: first row of the launch, q heads of one unit of work, resident CTAs
+    uint32_t row0, heads_at_once, workers;  // paged_tiles_kernel: first row of the launch, q heads of one unit of work, warps
     float scale;  // times log2(e)
 };
 
@@ -226,12 +226,11 @@ __global__ void __launch_bounds__(ROWS_THREADS) paged_rows_kernel(PagedAttnArgs 
         }
 }
 
-// One q head over a warp's share of the entries [t0, t1) of one kv head (16 of every 64, from `share` on) in plain f32: what the matrix instructions
-// cannot give where keys or values are not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions
+// One q head over the entries [t0, t1) of one kv head by one warp in plain f32: what the matrix instructions cannot give where keys or values are not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions
 // 2 lane, 2 lane + 1 (+ 64). Results as in paged_tiles_kernel.
 template <int HD>
-__device__ __noinline__ void paged_plain_share(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
-                                               uint32_t t1, uint32_t share, float bias, float* m_out, float* l_out, float* o_out) {
+__device__ __noinline__ void paged_plain_run(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
+                                             uint32_t t1, float bias, float* m_out, float* l_out, float* o_out) {
     const uint32_t lane = threadIdx.x & 31u, d = 2u * lane;
     const __half* K = reinterpret_cast<const __half*>(a.c.k);
     const __half* V = reinterpret_cast<const __half*>(a.c.v);
@@ -242,7 +241,6 @@ __device__ __noinline__ void paged_plain_share(const PagedAttnArgs& a, uint32_t 
         o[2 * j] = o[2 * j + 1] = 0.0f;
     }
     for (uint32_t e = t0; e < t1; ++e) {
-        if ((e & 63u) / 16u != share) continue;
         const uint32_t page = paged_page(a.c, slot, e);
         if (page == PAGED_NONE) continue;
         const size_t at = paged_row(a.c, page, kvh, e) + d;
@@ -282,32 +280,35 @@ __device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t sme
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
 }
 
-constexpr uint32_t TILE = 64, TILES_THREADS = 128;
+constexpr uint32_t TILE = 16, TILES_THREADS = 128, TILES_WARPS = TILES_THREADS / 32;
 // Weights are relative to the maximum less 15: f16 then holds a small one down to 2^-40 of the largest instead of 2^-25. That reference, as it is
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
 
-// The work of a launch is a list of tiles of 64 entries: rows in order, in a row the units of up to 8 (WIDE: 16) q heads of one kv head, in a unit
-// its tiles. Every resident CTA takes an equal run of the list, so that no CTA starts late and none ends early, whatever the lengths.
-// Each warp leaves its own (maximum, sum, output) of every unit that the run touches, without a barrier, and paged_join_kernel puts them together: the part
-// of CTA c in unit u of all units is number u + c, which no other has, as c or u grows from one part of the list to the next. Against one CTA per (row, unit, 1024 entries): 32 rows of up to 16384 entries 198 -> @A us,
-// one of 130001 110 -> @B.
-//   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units. A warp takes 16 entries.
+// The work of a launch is a list of tiles of 16 entries: rows in order, in a row the units of up to 8 (WIDE: 16) q heads of one kv head, in a unit
+// its tiles. Every warp takes an equal run of the list, with a ring of its own and without a barrier, so that no warp waits for another, none starts late and
+// none ends early, whatever the lengths. A warp leaves a part (maximum, sum, output) of every unit that its run touches, and paged_join_kernel puts the parts
+// together: the part of warp w in unit u of all units is number u + w, which no other has, as w or u grows from one part of the list to the next. Against one
+// CTA per (row, unit, 1024 entries) with barriers: 32 rows of up to 16384 entries 198 -> @A us, one of 130001 110 -> @B.
+//   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units.
 //   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them. A group has
 //                         at most 8 heads as a rule: hi and lo are then the two halves of the 16 rows of ONE operand, and the halves of the result are
 //                         added (WIDE: two products).
-//   softmax               online in base 2 per warp; the outputs are rescaled only when a maximum moved.
+//   softmax               online in base 2; the outputs are rescaled only when a maximum moved.
 constexpr uint32_t TILES_ROWS = 256;  // rows of a launch: their ranges stay in shared memory
 
-// The CTA whose run holds tile x of `total`; CTA i has [i total / n, (i + 1) total / n).
-__device__ __forceinline__ uint32_t cta_of(uint64_t x, uint64_t total, uint32_t n) { return (uint32_t)(((x + 1u) * n - 1u) / total); }
-__device__ __forceinline__ uint32_t ctas_at_work(uint64_t total, uint32_t n) { return total < n ? (uint32_t)total : n; }
+// The warp whose run holds tile x of `total`; warp i of n has [i total / n, (i + 1) total / n).
+__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t y) {  // most lists are short enough for the fast division
+    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
+}
+__device__ __forceinline__ uint32_t warp_of(uint64_t x, uint64_t total, uint32_t n) { return (uint32_t)quotient((x + 1u) * n - 1u, total); }
+__device__ __forceinline__ uint32_t warps_at_work(uint64_t total, uint32_t n) { return total < n ? (uint32_t)total : n; }
 
 template <int HD, bool WIDE>
 struct TilesCfg {
     static constexpr int STAGES = HD == 128 ? 3 : 4, CTAS = HD == 128 ? 2 : 3;
-    static constexpr int RING = STAGES * 2 * (int)TILE * HD * 2;
-    static constexpr int SMEM = 256 + RING + (int)(TILES_ROWS + 1) * 8 + (int)TILES_ROWS * 12;  // ring, the prefix, the rows' ranges
+    static constexpr int STAGE = 2 * (int)TILE * HD * 2;                                                                    // K and V of a tile
+    static constexpr int SMEM = 256 + (int)TILES_WARPS * STAGES * STAGE + (int)(TILES_ROWS + 1) * 8 + (int)TILES_ROWS * 12;  // rings, the prefix, the rows' ranges
 };
 
 template <int HD, bool WIDE>
@@ -315,15 +316,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     using Cfg = TilesCfg<HD, WIDE>;
     constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = Cfg::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t s_bad;
-    const uint32_t ring = ((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u;  // whole rows, for the exclusive or below
-    uint64_t* s_prefix = reinterpret_cast<uint64_t*>(smem + 256 + Cfg::RING);
+    uint64_t* s_prefix = reinterpret_cast<uint64_t*>(smem + 256 + TILES_WARPS * STAGES * Cfg::STAGE);
     uint32_t* s_slot = reinterpret_cast<uint32_t*>(s_prefix + TILES_ROWS + 1);
     uint32_t* s_begin = s_slot + TILES_ROWS;
     uint32_t* s_end = s_begin + TILES_ROWS;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
     const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = min(a.rows - a.row0, TILES_ROWS);
-    if (tid == 0) s_bad = 0u;
     pdl_wait();
     pdl_trigger();
     if (tid < 32u) {  // the rows' tiles, summed up by one warp
@@ -334,12 +332,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             if (r < rows) {
                 const bool inside = paged_row_range(a, a.row0 + r, &slot, &begin, &end);
                 if (!inside && blockIdx.x == 0) atomicOr(a.status, 1u);
-                n = inside && end > begin ? (end - (begin & ~63u) + 63u) / 64u : 0u;
+                n = inside && end > begin ? (end - (begin & ~(TILE - 1u)) + TILE - 1u) / TILE : 0u;
             }
-            uint64_t sum = n;
+            uint32_t sum = n;  // 32 rows of at most 2^26 tiles
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t u = __shfl_up_sync(0xffffffffu, sum, o);
+                const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= (uint32_t)o) sum += u;
             }
             if (r < rows) {
@@ -356,18 +354,18 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     }
     __syncthreads();
     const uint64_t total = s_prefix[rows] * units;
-    const uint32_t n_ctas = ctas_at_work(total, a.ctas);
-    if (blockIdx.x >= n_ctas) return;
-    const uint64_t lo = blockIdx.x * total / n_ctas;
-    const uint32_t count = (uint32_t)((blockIdx.x + 1u) * total / n_ctas - lo);  // at least 1
+    const uint32_t worker = blockIdx.x * TILES_WARPS + warp, workers = warps_at_work(total, a.workers);
+    if (worker >= workers) return;
+    const uint64_t lo = quotient(worker * total, workers);
+    const uint32_t count = (uint32_t)(quotient((worker + 1u) * total, workers) - lo);  // at least 1
 
     // a place in the list
     struct Place {
         uint32_t row, unit, tile, tiles, t0, t1, first;
     };
     auto enter = [&](Place& p) {  // p.row has tiles
-        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~63u;
-        p.tiles = (p.t1 - p.first + 63u) / 64u;
+        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~(TILE - 1u);
+        p.tiles = (p.t1 - p.first + TILE - 1u) / TILE;
     };
     auto advance = [&](Place& p) {
         if (++p.tile < p.tiles) return false;
@@ -390,60 +388,54 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         at.row = l;
         enter(at);
         const uint64_t in_row = lo - s_prefix[l] * units;
-        at.unit = (uint32_t)(in_row / at.tiles);
+        at.unit = (uint32_t)quotient(in_row, at.tiles);
         at.tile = (uint32_t)(in_row - (uint64_t)at.unit * at.tiles);
     }
 
-    constexpr uint32_t ROWS_AT_ONCE = TILES_THREADS / CHUNKS, COPIES = TILE / ROWS_AT_ONCE;  // a thread's rows lie a multiple of 8 apart: one swizzle for all
+    // The lane copies piece `ch` of rows my_row, my_row + ROWS_AT_ONCE, ..; the swizzle of row r is r mod 8.
+    constexpr uint32_t ROWS_AT_ONCE = 32u / CHUNKS, COPIES = TILE / ROWS_AT_ONCE, toSV = TILE * HD * 2u;
+    const uint32_t ring = (((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u) + warp * (STAGES * Cfg::STAGE);  // whole rows, for the exclusive or below
     const uint32_t subgroups = units / a.c.kv_heads;
-    const uint32_t in_page = (1u << a.c.shift) - 1u, my_row = tid / CHUNKS, ch = tid % CHUNKS;
+    const uint32_t in_page = (1u << a.c.shift) - 1u, my_row = lane / CHUNKS, ch = lane % CHUNKS;
     const uint64_t head_bytes = (uint64_t)(HD * 2u) << a.c.shift;
     const uint64_t page_bytes = a.c.kv_heads * head_bytes;
     const ptrdiff_t toV = a.c.v - a.c.k;
-    const uint32_t toSV = STAGES * TILE * HD * 2u;
-    const uint32_t my_dst = ring + my_row * (HD * 2u) + ((ch ^ (my_row & 7u)) * 16u);
+    const uint32_t my_dst = ring + my_row * (HD * 2u) + ((ch ^ my_row) * 16u);  // my_row < 8; c * ROWS_AT_ONCE enters by exclusive or
     Place fetch = at;
     const uint32_t* pages = nullptr;
     const unsigned char* srcK = nullptr;
+    bool bad = false;  // the warp met a page outside the pool
     auto aim = [&]() {
         pages = a.c.table + (size_t)s_slot[fetch.row] * a.c.max_pages;
         srcK = a.c.k + fetch.unit / subgroups * head_bytes + ch * 16u;
     };
     auto load = [&](uint32_t f) {  // tile f of the run, where `fetch` is
-        const uint32_t base = fetch.first + fetch.tile * TILE, dst = my_dst + (f % STAGES) * (TILE * HD * 2u);
-        if (base < fetch.t0 || base + TILE > fetch.t1) {
-            for (uint32_t c = 0; c < COPIES; ++c) {
-                const uint32_t e = base + c * ROWS_AT_ONCE + my_row, pg = e >= fetch.t0 && e < fetch.t1 ? pages[e >> a.c.shift] : PAGED_NONE;
-                const bool ok = pg < a.c.pages;
-                if (!ok && e >= fetch.t0 && e < fetch.t1) s_bad = 1u;
-                const unsigned char* src = ok ? srcK + pg * page_bytes + (e & in_page) * (HD * 2u) : a.c.k;
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, ok ? src + toV : a.c.v, ok ? 16u : 0u);
-            }
-        } else if (a.c.shift >= 6u) {  // a tile within one page
+        const uint32_t base = fetch.first + fetch.tile * TILE, dst = my_dst + (f % STAGES) * Cfg::STAGE;
+        if (a.c.shift >= 4u && base >= fetch.t0 && base + TILE <= fetch.t1) {  // a whole tile, within one page
             const uint32_t pg = pages[base >> a.c.shift];
             const bool ok = pg < a.c.pages;
-            if (!ok) s_bad = 1u;
+            bad |= !ok;
             const unsigned char* src = srcK + (ok ? pg * page_bytes : 0) + ((base & in_page) + my_row) * (HD * 2u);
             const unsigned char* srcV = src + toV;
             const uint32_t bytes = ok ? 16u : 0u;
 #pragma unroll
             for (uint32_t c = 0; c < COPIES; ++c) {
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src + c * (ROWS_AT_ONCE * HD * 2u), bytes);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, srcV + c * (ROWS_AT_ONCE * HD * 2u), bytes);
+                const uint32_t to = (dst ^ ((c * ROWS_AT_ONCE & 7u) * 16u)) + c * (ROWS_AT_ONCE * HD * 2u);
+                cp_async16_or_zero(to, src + c * (ROWS_AT_ONCE * HD * 2u), bytes);
+                cp_async16_or_zero(to + toSV, srcV + c * (ROWS_AT_ONCE * HD * 2u), bytes);
             }
         } else {
-            uint32_t page[COPIES];
-#pragma unroll
-            for (uint32_t c = 0; c < COPIES; ++c) page[c] = pages[(base + c * ROWS_AT_ONCE + my_row) >> a.c.shift];  // all lookups on their way together
-#pragma unroll
+#pragma unroll 1
             for (uint32_t c = 0; c < COPIES; ++c) {
                 const uint32_t e = base + c * ROWS_AT_ONCE + my_row;
-                const bool ok = page[c] < a.c.pages;
-                if (!ok) s_bad = 1u;
-                const unsigned char* src = srcK + (ok ? page[c] * page_bytes : 0) + (e & in_page) * (HD * 2u);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u), src, ok ? 16u : 0u);
-                cp_async16_or_zero(dst + c * (ROWS_AT_ONCE * HD * 2u) + toSV, src + toV, ok ? 16u : 0u);
+                const bool in = e >= fetch.t0 && e < fetch.t1;
+                const uint32_t pg = in ? pages[e >> a.c.shift] : PAGED_NONE;
+                const bool ok = pg < a.c.pages;
+                bad |= in && !ok;
+                const unsigned char* src = ok ? srcK + pg * page_bytes + (e & in_page) * (HD * 2u) : a.c.k;
+                const uint32_t to = (dst ^ ((c * ROWS_AT_ONCE & 7u) * 16u)) + c * (ROWS_AT_ONCE * HD * 2u);
+                cp_async16_or_zero(to, src, ok ? 16u : 0u);
+                cp_async16_or_zero(to + toSV, ok ? src + toV : a.c.v, ok ? 16u : 0u);
             }
         }
         if (advance(fetch) && f + 1u < count) aim();
@@ -456,7 +448,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     }
 
     // ldmatrix: the lane's row and 16-byte piece; the pieces of a product step follow by exclusive or
-    const uint32_t mj = lane >> 3, kr = warp * 16 + (mj >> 1) * 8 + (lane & 7u), vr = warp * 16 + (mj & 1u) * 8 + (lane & 7u);
+    const uint32_t mj = lane >> 3, kr = (mj >> 1) * 8 + (lane & 7u), vr = (mj & 1u) * 8 + (lane & 7u);
     const uint32_t k_at = ring + kr * (HD * 2u) + (((mj & 1u) ^ (kr & 7u)) * 16u);
     const uint32_t v_at = ring + toSV + vr * (HD * 2u) + (((mj >> 1) ^ (vr & 7u)) * 16u);
     constexpr int H = WIDE ? 2 : 1;  // heads of a thread
@@ -495,10 +487,11 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
         }
         cp_async_wait<STAGES - 2>();
-        __syncthreads();
+        __syncwarp();
+        // the stage that is filled again was read by products that have been issued: their operands are in registers
         if (f + STAGES - 1 < count) load(f + STAGES - 1);
         cp_async_commit();
-        const uint32_t stage = (f % STAGES) * (TILE * HD * 2u);
+        const uint32_t stage = (f % STAGES) * Cfg::STAGE;
         float s0[2][4], s1[2][4];  // even and odd product steps: two short chains each
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] = s0[1][i] = s1[0][i] = s1[1][i] = 0.0f;
@@ -514,7 +507,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             }
         }
         // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
-        const uint32_t base = at.first + at.tile * TILE, e0 = base + warp * 16 + 2 * t4;
+        const uint32_t base = at.first + at.tile * TILE, e0 = base + 2 * t4;
         float s[H][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] += s0[1][i], s1[0][i] += s1[1][i];
@@ -523,13 +516,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             s[h][0] = WIDE ? s0[0][2 * h] : s0[0][0] + s0[0][2], s[h][1] = WIDE ? s0[0][2 * h + 1] : s0[0][1] + s0[0][3];
             s[h][2] = WIDE ? s1[0][2 * h] : s1[0][0] + s1[0][2], s[h][3] = WIDE ? s1[0][2 * h + 1] : s1[0][1] + s1[0][3];
         }
-        const bool bad = *(volatile uint32_t*)&s_bad != 0u;
-        if (base < at.t0 || base + TILE > at.t1 || bad) {
+        if (base < at.t0 || base + TILE > at.t1 || __any_sync(0xffffffffu, bad)) {
             const uint32_t* own_pages = a.c.table + (size_t)s_slot[at.row] * a.c.max_pages;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
-                if (e < at.t0 || e >= at.t1 || (bad && own_pages[e >> a.c.shift] >= a.c.pages)) {
+                if (e < at.t0 || e >= at.t1 || own_pages[e >> a.c.shift] >= a.c.pages) {
 #pragma unroll
                     for (int h = 0; h < H; ++h) s[h][i] = -INFINITY;
                 }
@@ -589,7 +581,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         if (ends || f + 1u == count) {
             // this warp's part of the unit
             const uint32_t row = a.row0 + at.row, kvh = at.unit / subgroups;
-            const size_t part = (((size_t)at.row * units + at.unit + blockIdx.x) * 4u + warp) * a.heads_at_once;
+            const size_t part = ((size_t)at.row * units + at.unit + worker) * a.heads_at_once;
             bool fine[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
@@ -617,8 +609,8 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                     odd &= ~(0xfu << (4u * gh));
                     const size_t at_part = part + gh + 8u * h, at_head = (size_t)row * a.q_heads + head;
                     __syncwarp();
-                    paged_plain_share<HD>(a, s_slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
-                                          max(at.t0, at.first + tile_begin * TILE), min(at.t1, base + TILE), warp, WEIGHT_BIAS, a.part_m + at_part,
+                    paged_plain_run<HD>(a, s_slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
+                                          max(at.t0, at.first + tile_begin * TILE), min(at.t1, base + TILE), WEIGHT_BIAS, a.part_m + at_part,
                                           a.part_l + at_part, a.part_o + at_part * HD);
                 }
             }
@@ -626,16 +618,17 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         entering = advance(at);
     }
     cp_async_wait<0>();
-    if (s_bad && tid == 0) atomicOr(a.status, 1u);
+    if (bad) atomicOr(a.status, 1u);
 }
 
-// The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most 1792: four warps of 444 CTAs); then eight groups of lanes take every
-// eighth part, each lane its dimensions, and the groups' sums meet in shared memory.
-template <int V, typename Part>
+// The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most 1792, the warps of 444 CTAs);
+// then 256 / LANES groups of lanes take every so-many-th part, each lane V dimensions, and the groups' sums meet in shared memory. CTAs of 8 lanes share a
+// head's dimensions where there are few heads, for more loads at a time.
+template <int V, int LANES, typename Part>
 __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t parts, Part part) {
-    constexpr uint32_t MOST = 1792;
+    constexpr uint32_t MOST = 1792, GROUPS = 256 / LANES;
     __shared__ float sw[MOST], red[16];
-    __shared__ float s_acc[8][32 * V];
+    __shared__ float s_acc[GROUPS][LANES * V];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
     float m[MOST / 256], l[MOST / 256], M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -668,56 +661,50 @@ __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t 
     L = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) L += red[8 + i];
-    if (a.stat && tid == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
-    for (uint32_t d0 = 0; d0 < hd; d0 += 32u * V) {
-        float acc[V];
+    if (a.stat && tid == 0 && blockIdx.z == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+    const uint32_t vl = tid % LANES, group = tid / LANES, d = (blockIdx.z * LANES + vl) * V;
+    float acc[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-        const uint32_t d = d0 + V * lane;
-        if (d < hd) {
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    if (d < hd) {
 #pragma unroll 4
-            for (uint32_t s = warp; s < parts; s += 8u) {
-                const float w = sw[s];
-                const float* src = a.part_o + part(s) * hd + d;
-                float x[V];
-                if constexpr (V == 4) {
-                    const float4 y = *reinterpret_cast<const float4*>(src);
-                    x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[i] = src[i];
-                }
-                if (w != 0.0f)  // an empty part's outputs may be anything
-#pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[i], acc[i]);
+        for (uint32_t s = group; s < parts; s += GROUPS) {
+            const float w = sw[s];
+            const float* src = a.part_o + part(s) * hd + d;
+            float x[V];
+            if constexpr (V == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src);
+                x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+            } else {
+                x[0] = src[0];
             }
+            if (w != 0.0f)  // an empty part's outputs may be anything
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[i], acc[i]);
         }
+    }
 #pragma unroll
-        for (int i = 0; i < V; ++i) s_acc[warp][i * 32 + lane] = acc[i];
-        __syncthreads();
-        if (warp == 0 && d < hd) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float o = s_acc[0][i * 32 + lane];
-#pragma unroll
-                for (int w = 1; w < 8; ++w) o += s_acc[w][i * 32 + lane];
-                a.out[head * hd + d + i] = L == 0.0f ? 0.0f : o / L;
-            }
-        }
-        __syncthreads();
+    for (int i = 0; i < V; ++i) s_acc[group][i * LANES + vl] = acc[i];
+    __syncthreads();
+    if (tid < LANES * V) {  // value tid: i = tid / LANES of lane tid % LANES
+        const uint32_t at = (blockIdx.z * LANES + tid % LANES) * V + tid / LANES;
+        float o = 0.0f;
+        for (int g = 0; g < (int)GROUPS; ++g) o += s_acc[g][tid];
+        if (at < hd) a.out[head * hd + at] = L == 0.0f ? 0.0f : o / L;
     }
 }
 
 // Parts of paged_rows_kernel: [row][q head][split].
-template <int V>
+template <int V, int LANES>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
     pdl_wait();
     pdl_trigger();
     const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
-    paged_join_parts<V>(a, head, a.splits, [=](uint32_t s) { return base + s; });
+    paged_join_parts<V, LANES>(a, head, a.splits, [=](uint32_t s) { return base + s; });
 }
 
-// Parts of paged_tiles_kernel, and the zeros of rows without entries. Grid (q head, row of the launch).
+// Parts of paged_tiles_kernel, and the zeros of rows without entries. Grid (q head, row of the launch, share of the dimensions).
+template <int LANES>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
     pdl_wait();
     pdl_trigger();
@@ -727,14 +714,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
     const size_t head = (size_t)(a.row0 + r) * a.q_heads + blockIdx.x;
     const uint64_t before = a.prefix[r], tiles = a.prefix[r + 1] - before, total = a.prefix[rows] * units;
     if (tiles == 0) {
-        for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
+        if (blockIdx.z == 0)
+            for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
         return;
     }
-    const uint32_t n = ctas_at_work(total, a.ctas);
+    const uint32_t n = warps_at_work(total, a.workers);
     const uint64_t lo = before * units + unit * tiles;
-    const uint32_t c0 = cta_of(lo, total, n), c1 = cta_of(lo + tiles - 1u, total, n);
-    const size_t part = ((size_t)r * units + unit + c0) * 4u;  // four warps' parts for every CTA
-    paged_join_parts<4>(a, head, 4u * (c1 - c0 + 1u), [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
+    const uint32_t w0 = warp_of(lo, total, n), w1 = warp_of(lo + tiles - 1u, total, n);
+    const size_t part = (size_t)r * units + unit + w0;
+    paged_join_parts<4, LANES>(a, head, w1 - w0 + 1u, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
 }
 
 // CTA = (256 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
@@ -770,16 +758,24 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a) {
     a.weights_out[at] = w;
 }
 
+// Whether a CTA per head and row leaves most of the device idle.
+bool few_heads(const M40llmCudaContext* ctx, uint32_t q_heads, uint32_t rows) { return (uint64_t)q_heads * rows <= 2ull * (uint64_t)ctx->sm_count; }
+
 // All rows in launches of up to 256, each followed by its join.
 template <int HD, bool WIDE>
 cudaError_t launch_tiles(M40llmCudaContext* ctx, PagedAttnArgs a) {
     using Cfg = TilesCfg<HD, WIDE>;
     cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-    a.ctas = (uint32_t)ctx->sm_count * Cfg::CTAS;
+    const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + TILE - 1u) / TILE) * a.rows;
+    a.workers = (uint32_t)ctx->sm_count * Cfg::CTAS * TILES_WARPS;
+    if (most < a.workers) a.workers = (uint32_t)most;
     for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += TILES_ROWS) {
         const uint32_t rows = a.rows - a.row0 < TILES_ROWS ? a.rows - a.row0 : TILES_ROWS;
-        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.ctas), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
-        if (e == cudaSuccess) e = m40_launch_dependent(paged_join_kernel, dim3(a.q_heads, rows), dim3(256), 0, ctx->decode_stream, a);
+        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3((a.workers + TILES_WARPS - 1u) / TILES_WARPS), dim3(TILES_THREADS), Cfg::SMEM,
+                                 ctx->decode_stream, a);
+        if (e == cudaSuccess)
+            e = few_heads(ctx, a.q_heads, rows) ? m40_launch_dependent(paged_join_kernel<8>, dim3(a.q_heads, rows, HD / 32), dim3(256), 0, ctx->decode_stream, a)
+                                                : m40_launch_dependent(paged_join_kernel<32>, dim3(a.q_heads, rows), dim3(256), 0, ctx->decode_stream, a);
         M40_COUNT_LAUNCH(ctx);
         M40_COUNT_LAUNCH(ctx);
     }
@@ -844,7 +840,7 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     if (tiles || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? a.bound : 0u;
         const size_t rows_at_once = c->rows < TILES_ROWS ? c->rows : TILES_ROWS;
-        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u)) * 4u * a.heads_at_once
+        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u) * TILES_WARPS) * a.heads_at_once
                                    : heads * a.splits;
         const size_t floats = parts * (hd + 2) + heads * 2 + heads * (size_t)a.ld_scores;
         const size_t prefix = (TILES_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
@@ -884,8 +880,12 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
                           : launch_rows<__half, 1>(a, grid, T, vec, pitch, smem, s);
         M40_COUNT_LAUNCH(ctx);
         if (e == cudaSuccess && (a.splits > 1 || a.scores)) {
-            e = hd % 4u == 0 ? m40_launch_dependent(paged_merge_kernel<4>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a)
-                             : m40_launch_dependent(paged_merge_kernel<1>, dim3(c->q_heads, c->rows), dim3(256), 0, s, a);
+            if (hd % 4u != 0)
+                e = m40_launch_dependent(paged_merge_kernel<1, 32>, dim3(c->q_heads, c->rows, (hd + 31u) / 32u), dim3(256), 0, s, a);
+            else if (few_heads(ctx, c->q_heads, c->rows))
+                e = m40_launch_dependent(paged_merge_kernel<4, 8>, dim3(c->q_heads, c->rows, (hd + 31u) / 32u), dim3(256), 0, s, a);
+            else
+                e = m40_launch_dependent(paged_merge_kernel<4, 32>, dim3(c->q_heads, c->rows, (hd + 127u) / 128u), dim3(256), 0, s, a);
             M40_COUNT_LAUNCH(ctx);
         }
     }
