@@ -226,11 +226,13 @@ __global__ void __launch_bounds__(ROWS_THREADS) paged_rows_kernel(PagedAttnArgs 
         }
 }
 
+constexpr uint32_t TILE = 16, TILES_THREADS = 128, TILES_WARPS = TILES_THREADS / 32, SPAN = TILE * TILES_WARPS;
+
 // One q head over the entries [t0, t1) of one kv head by one warp in plain f32: what the matrix instructions cannot give where keys or values are not finite (a part of 0, or of the other sign, times an infinity is NaN). Lane = dimensions
 // 2 lane, 2 lane + 1 (+ 64). Results as in paged_tiles_kernel.
 template <int HD>
 __device__ __noinline__ void paged_plain_run(const PagedAttnArgs& a, uint32_t slot, uint32_t kvh, const float* q, float* scores, uint32_t t0,
-                                             uint32_t t1, float bias, float* m_out, float* l_out, float* o_out) {
+                                             uint32_t t1, uint32_t share, float bias, float* m_out, float* l_out, float* o_out) {
     const uint32_t lane = threadIdx.x & 31u, d = 2u * lane;
     const __half* K = reinterpret_cast<const __half*>(a.c.k);
     const __half* V = reinterpret_cast<const __half*>(a.c.v);
@@ -241,6 +243,7 @@ __device__ __noinline__ void paged_plain_run(const PagedAttnArgs& a, uint32_t sl
         o[2 * j] = o[2 * j + 1] = 0.0f;
     }
     for (uint32_t e = t0; e < t1; ++e) {
+        if (e / TILE % TILES_WARPS != share) continue;
         const uint32_t page = paged_page(a.c, slot, e);
         if (page == PAGED_NONE) continue;
         const size_t at = paged_row(a.c, page, kvh, e) + d;
@@ -280,7 +283,6 @@ __device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t sme
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
 }
 
-constexpr uint32_t TILE = 16, TILES_THREADS = 128, TILES_WARPS = TILES_THREADS / 32;
 // Weights are relative to the maximum less 15: f16 then holds a small one down to 2^-40 of the largest instead of 2^-25. That reference, as it is
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             if (r < rows) {
                 const bool inside = paged_row_range(a, a.row0 + r, &slot, &begin, &end);
                 if (!inside && blockIdx.x == 0) atomicOr(a.status, 1u);
-                n = inside && end > begin ? (end - (begin & ~(TILE - 1u)) + TILE - 1u) / TILE : 0u;
+                n = inside && end > begin ? (end - (begin & ~(SPAN - 1u)) + SPAN - 1u) / SPAN : 0u;
             }
             uint32_t sum = n;  // 32 rows of at most 2^26 tiles
 #pragma unroll
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     }
     __syncthreads();
     const uint64_t total = s_prefix[rows] * units;
-    const uint32_t worker = blockIdx.x * TILES_WARPS + warp, workers = warps_at_work(total, a.workers);
+    const uint32_t worker = blockIdx.x, workers = warps_at_work(total, a.workers);
     if (worker >= workers) return;
     const uint64_t lo = quotient(worker * total, workers);
     const uint32_t count = (uint32_t)(quotient((worker + 1u) * total, workers) - lo);  // at least 1
@@ -364,8 +366,8 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         uint32_t row, unit, tile, tiles, t0, t1, first;
     };
     auto enter = [&](Place& p) {  // p.row has tiles
-        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~(TILE - 1u);
-        p.tiles = (p.t1 - p.first + TILE - 1u) / TILE;
+        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~(SPAN - 1u);
+        p.tiles = (p.t1 - p.first + SPAN - 1u) / SPAN;
     };
     auto advance = [&](Place& p) {
         if (++p.tile < p.tiles) return false;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         srcK = a.c.k + fetch.unit / subgroups * head_bytes + ch * 16u;
     };
     auto load = [&](uint32_t f) {  // tile f of the run, where `fetch` is
-        const uint32_t base = fetch.first + fetch.tile * TILE, dst = my_dst + (f % STAGES) * Cfg::STAGE;
+        const uint32_t base = fetch.first + fetch.tile * SPAN + warp * TILE, dst = my_dst + (f % STAGES) * Cfg::STAGE;
         if (a.c.shift >= 4u && base >= fetch.t0 && base + TILE <= fetch.t1) {  // a whole tile, within one page
             const uint32_t pg = pages[base >> a.c.shift];
             const bool ok = pg < a.c.pages;
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                 cp_async16_or_zero(to, src + c * (ROWS_AT_ONCE * HD * 2u), bytes);
                 cp_async16_or_zero(to + toSV, srcV + c * (ROWS_AT_ONCE * HD * 2u), bytes);
             }
-        } else {
+        } else if (base < fetch.t1 && base + TILE > fetch.t0) {
 #pragma unroll 1
             for (uint32_t c = 0; c < COPIES; ++c) {
                 const uint32_t e = base + c * ROWS_AT_ONCE + my_row;
@@ -487,11 +489,13 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             for (int h = 0; h < H; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
         }
         cp_async_wait<STAGES - 2>();
-        __syncwarp();
+        __syncthreads();
         // the stage that is filled again was read by products that have been issued: their operands are in registers
         if (f + STAGES - 1 < count) load(f + STAGES - 1);
         cp_async_commit();
         const uint32_t stage = (f % STAGES) * Cfg::STAGE;
+        const uint32_t base = at.first + at.tile * SPAN + warp * TILE, e0 = base + 2 * t4;
+        if (base < at.t1 && base + TILE > at.t0) {
         float s0[2][4], s1[2][4];  // even and odd product steps: two short chains each
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] = s0[1][i] = s1[0][i] = s1[1][i] = 0.0f;
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             }
         }
         // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
-        const uint32_t base = at.first + at.tile * TILE, e0 = base + 2 * t4;
+        
         float s[H][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] += s0[1][i], s1[0][i] += s1[1][i];
@@ -531,10 +535,11 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
-                    if (g + 8u * h < G && e >= at.t0 && e < at.t1)
-                        a.scores[((size_t)(a.row0 + at.row) * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e] = s[h][i];
+                for (int i = 0; i < 2; ++i) {  // entries outside the row's are not read again
+                    const uint32_t e = e0 + 8u * i;
+                    if (g + 8u * h < G && e < a.ld_scores)
+                        *reinterpret_cast<float2*>(a.scores + ((size_t)(a.row0 + at.row) * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e) =
+                            make_float2(s[h][2 * i], s[h][2 * i + 1]);
                 }
         }
         uint32_t ph[H][2], pl[H][2];
@@ -577,11 +582,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             }
         }
 
+        }
         const bool ends = at.tile + 1u == at.tiles;
         if (ends || f + 1u == count) {
             // this warp's part of the unit
             const uint32_t row = a.row0 + at.row, kvh = at.unit / subgroups;
-            const size_t part = ((size_t)at.row * units + at.unit + worker) * a.heads_at_once;
+            const size_t part = (((size_t)at.row * units + at.unit + worker) * TILES_WARPS + warp) * a.heads_at_once;
             bool fine[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
@@ -610,7 +616,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                     const size_t at_part = part + gh + 8u * h, at_head = (size_t)row * a.q_heads + head;
                     __syncwarp();
                     paged_plain_run<HD>(a, s_slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
-                                          max(at.t0, at.first + tile_begin * TILE), min(at.t1, base + TILE), WEIGHT_BIAS, a.part_m + at_part,
+                                          max(at.t0, at.first + tile_begin * SPAN), min(at.t1, at.first + (at.tile + 1u) * SPAN), warp, WEIGHT_BIAS, a.part_m + at_part,
                                           a.part_l + at_part, a.part_o + at_part * HD);
                 }
             }
@@ -721,41 +727,93 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
     const uint32_t n = warps_at_work(total, a.workers);
     const uint64_t lo = before * units + unit * tiles;
     const uint32_t w0 = warp_of(lo, total, n), w1 = warp_of(lo + tiles - 1u, total, n);
-    const size_t part = (size_t)r * units + unit + w0;
-    paged_join_parts<4, LANES>(a, head, w1 - w0 + 1u, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
+    const size_t part = ((size_t)r * units + unit + w0) * TILES_WARPS;
+    paged_join_parts<4, LANES>(a, head, (w1 - w0 + 1u) * TILES_WARPS, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
 }
 
-// CTA = (256 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
-// depend on who comes first.
-__global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a) {
+// CTA = (1024 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
+// depend on who comes first. Thread = four neighbouring entries (one after the other where weights or scores are not 16-byte aligned).
+// Bound by the scores, which mostly come out of L2.
+constexpr uint32_t WEIGHTS_AT_ONCE = 1024;
+__global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uint32_t vec) {
+    __shared__ uint32_t s_most, s_count, s_row[256];
     pdl_wait();
     pdl_trigger();
-    const uint32_t row = blockIdx.z, h = blockIdx.y, e = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t tid = threadIdx.x, row = blockIdx.z, h = blockIdx.y;
     const uint32_t slot = a.row_slot[row];
     if (slot >= a.c.slots) return;
-    uint32_t most = 0, skip = 0;
-    for (uint32_t r = 0; r < a.rows; ++r) {
+    if (tid == 0) s_most = 0u, s_count = 0u;
+    __syncthreads();
+    bool skip = false;
+    uint32_t most = 0;
+    for (uint32_t r = tid; r < a.rows; r += 256u) {
         uint32_t s, b, n;
         const bool inside = paged_row_range(a, r, &s, &b, &n);
         if (s != slot) continue;
-        if (r < row || !inside) skip = 1;
+        if (r < row || !inside) skip = true;
         most = max(most, n);
     }
-    if (skip || e >= most) return;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31u) == 0 && most) atomicMax(&s_most, most);
+    if (__syncthreads_or(skip)) return;
+    most = s_most;
+    const uint32_t e = blockIdx.x * WEIGHTS_AT_ONCE + 4u * tid;
+    if (blockIdx.x * WEIGHTS_AT_ONCE >= most) return;
     const size_t at = ((size_t)slot * a.c.kv_heads + h) * a.ld_weights + e;
-    float w = a.weights_in ? a.weights_in[at] : 0.0f;
-    for (uint32_t r = row; r < a.rows; ++r) {
-        uint32_t s, b, n;
-        paged_row_range(a, r, &s, &b, &n);
-        if (s != slot || e < b || e >= n) continue;
-        float sum = 0.0f;
-        for (uint32_t g = 0; g < a.group; ++g) {
-            const size_t head = (size_t)r * a.q_heads + h * a.group + g;
-            sum += exp2f(a.scores[head * a.ld_scores + e] - a.stat[2 * head]) * a.stat[2 * head + 1];
-        }
-        w += sum;
+    const bool whole = vec && e + 4u <= most;
+    float w[4];
+    if (whole && a.weights_in) {
+        const float4 x = *reinterpret_cast<const float4*>(a.weights_in + at);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) w[i] = a.weights_in && e + i < most ? a.weights_in[at + i] : 0.0f;
     }
-    a.weights_out[at] = w;
+    for (uint32_t r0 = row; r0 < a.rows; r0 += 256u) {  // the slot's rows among the next 256, in order
+        const uint32_t r = r0 + tid, mine = r < a.rows && a.row_slot[r] == slot ? 1u : 0u;
+        __syncthreads();
+        if (tid == 0) s_count = 0u;
+        const uint32_t mask = __ballot_sync(0xffffffffu, mine);
+        for (uint32_t k = 0; k < 8u; ++k) {
+            __syncthreads();
+            if (tid / 32u == k && mask) {
+                if (mine) s_row[s_count + __popc(mask & ((1u << (tid & 31u)) - 1u))] = r;
+                __syncwarp();
+                if ((tid & 31u) == 0) s_count += __popc(mask);
+            }
+        }
+        __syncthreads();
+        for (uint32_t k = 0; k < s_count; ++k) {
+            uint32_t s, b, n;
+            paged_row_range(a, s_row[k], &s, &b, &n);
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const size_t head = (size_t)s_row[k] * a.q_heads + h * a.group;
+            const bool all = whole && e >= b && e + 4u <= n;
+#pragma unroll 4
+            for (uint32_t g = 0; g < a.group; ++g) {
+                const float M = a.stat[2 * (head + g)], inv = a.stat[2 * (head + g) + 1];
+                const float* sc = a.scores + (head + g) * a.ld_scores + e;
+                if (all) {
+                    const float4 x = *reinterpret_cast<const float4*>(sc);
+                    sum[0] += exp2f(x.x - M) * inv, sum[1] += exp2f(x.y - M) * inv;
+                    sum[2] += exp2f(x.z - M) * inv, sum[3] += exp2f(x.w - M) * inv;
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        if (e + i >= b && e + i < n) sum[i] += exp2f(sc[i] - M) * inv;
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) w[i] += sum[i];
+        }
+    }
+    if (whole) {
+        *reinterpret_cast<float4*>(a.weights_out + at) = make_float4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (e + i < most) a.weights_out[at + i] = w[i];
+    }
 }
 
 // Whether a CTA per head and row leaves most of the device idle.
@@ -766,12 +824,12 @@ template <int HD, bool WIDE>
 cudaError_t launch_tiles(M40llmCudaContext* ctx, PagedAttnArgs a) {
     using Cfg = TilesCfg<HD, WIDE>;
     cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-    const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + TILE - 1u) / TILE) * a.rows;
-    a.workers = (uint32_t)ctx->sm_count * Cfg::CTAS * TILES_WARPS;
+    const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + SPAN - 1u) / SPAN) * a.rows;
+    a.workers = (uint32_t)ctx->sm_count * Cfg::CTAS;
     if (most < a.workers) a.workers = (uint32_t)most;
     for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += TILES_ROWS) {
         const uint32_t rows = a.rows - a.row0 < TILES_ROWS ? a.rows - a.row0 : TILES_ROWS;
-        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3((a.workers + TILES_WARPS - 1u) / TILES_WARPS), dim3(TILES_THREADS), Cfg::SMEM,
+        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM,
                                  ctx->decode_stream, a);
         if (e == cudaSuccess)
             e = few_heads(ctx, a.q_heads, rows) ? m40_launch_dependent(paged_join_kernel<8>, dim3(a.q_heads, rows, HD / 32), dim3(256), 0, ctx->decode_stream, a)
@@ -838,11 +896,11 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     }
     const size_t heads = (size_t)c->rows * c->q_heads;
     if (tiles || a.splits > 1 || c->weights_out) {
-        a.ld_scores = c->weights_out ? a.bound : 0u;
+        a.ld_scores = c->weights_out ? (a.bound + 3u) & ~3u : 0u;
         const size_t rows_at_once = c->rows < TILES_ROWS ? c->rows : TILES_ROWS;
-        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u) * TILES_WARPS) * a.heads_at_once
+        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u)) * TILES_WARPS * a.heads_at_once
                                    : heads * a.splits;
-        const size_t floats = parts * (hd + 2) + heads * 2 + heads * (size_t)a.ld_scores;
+        const size_t floats = parts * (hd + 2) + heads * 2 + 4 + heads * (size_t)a.ld_scores;
         const size_t prefix = (TILES_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
         unsigned char* work_area = (unsigned char*)m40_ensure_scratch(ctx, 1, prefix + 8 + floats * sizeof(float), 0);
         if (!work_area) return -5;
@@ -852,7 +910,7 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         a.part_l = a.part_m + parts;
         if (c->weights_out) {
             a.stat = a.part_l + parts;
-            a.scores = a.stat + 2 * heads;
+            a.scores = a.part_o + ((parts * (hd + 2) + heads * 2 + 3) & ~(size_t)3);  // 16-byte aligned
         }
     }
     cudaError_t e;
@@ -890,7 +948,9 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         }
     }
     if (e == cudaSuccess && a.scores) {
-        e = m40_launch_dependent(paged_weights_kernel, dim3((a.bound + 255u) / 256u, cache->kv_heads, c->rows), dim3(256), 0, s, a);
+        const bool aligned = ((((uintptr_t)a.weights_in) | ((uintptr_t)a.weights_out) | ((uintptr_t)a.scores)) & 15u) == 0 && a.ld_weights % 4u == 0;
+        e = m40_launch_dependent(paged_weights_kernel, dim3((a.bound + WEIGHTS_AT_ONCE - 1u) / WEIGHTS_AT_ONCE, cache->kv_heads, c->rows), dim3(256), 0, s, a,
+                                 aligned ? 1u : 0u);
         M40_COUNT_LAUNCH(ctx);
     }
     if (e != cudaSuccess) {
