@@ -72,21 +72,26 @@ __device__ __forceinline__ Candidate warp_best(Candidate c) {
 
 constexpr uint32_t LP_LIST = 512;  // candidates that a CTA sorts by counting
 
+// Larger is better, as f32; for maxima by integer reductions.
+__device__ __forceinline__ uint32_t lp_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float lp_value(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
+
 // A sum of e = exp(x - m) and of e (x - m), m near the largest of its values (or -inf without any).
 struct Sums {
     float m, s, t;
 };
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), da = against(a.m, m), db = against(b.m, m);
-    const float ea = exp2_fast(da * LP_LOG2E), eb = exp2_fast(db * LP_LOG2E);
-    Sums r = {m, a.s * ea + b.s * eb, 0.0f};
-    if (ea > 0.0f) r.t += (a.t + da * a.s) * ea;
-    if (eb > 0.0f) r.t += (b.t + db * b.s) * eb;
-    return r;
+// `v` brought to reference m, the largest of the references that meet (a sum without values has the reference -inf).
+__device__ __forceinline__ Sums moved(const Sums& v, float m) {
+    const float d = against(v.m, m), e = exp2_fast(d * LP_LOG2E);
+    return Sums{m, v.s * e, e > 0.0f ? (v.t + d * v.s) * e : 0.0f};
 }
 __device__ __forceinline__ Sums warp_joined(Sums v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = joined(v, Sums{__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.t, o)});
+    v = moved(v, lp_value(__reduce_max_sync(0xffffffffu, lp_key(v.m))));
+    v.s = warp_sum(v.s);
+    v.t = warp_sum(v.t);
     return v;
 }
 // two values at a time
@@ -122,13 +127,6 @@ struct Share {
     uint32_t ahead;
     Candidate list[LP_TOP_MAX];
 };
-
-// Larger is better, as f32; for maxima by integer reductions.
-__device__ __forceinline__ uint32_t lp_key(float x) {
-    const uint32_t b = __float_as_uint(x + 0.0f);
-    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float lp_value(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key); }
 
 // Cluster = one row (one CTA as a rule), CTA c has the values [c * per, (c + 1) * per). The row is read once, with four 16-byte loads of a thread on their way together.
 //   sums      every thread keeps a reference m, moved only when a value is more than 16 above it, so that exp(x - m) needs no second pass and no rescaling as a
@@ -196,10 +194,7 @@ __global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32
         take2(v, -INFINITY, pair_of(-m, -m));
         if (ranked) above += v >= (i < split ? reach : beyond);
     }
-    for (uint32_t j0 = tid; j0 < fours; j0 += AT_ONCE * T) {
-        float4 v[AT_ONCE];
-#pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = j0 + k * T < fours ? x4[j0 + k * T] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const auto take = [&](const float4 (&v)[AT_ONCE], uint32_t j0) {
         float largest = -INFINITY;  // NaN falls out
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; ++k) largest = fmaxf(fmaxf(largest, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
@@ -207,25 +202,40 @@ __global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32
         move_to(largest);
         const uint64_t minus_m = pair_of(-m, -m);
 #pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; ++k) {
-            take2(v[k].x, v[k].y, minus_m);
-            take2(v[k].z, v[k].w, minus_m);
-            if (ranked) {
-                const uint32_t i = head + 4u * (j0 + k * T);
-                const float level = i < split ? reach : beyond;
-                above += v[k].x >= level, above += v[k].y >= level, above += v[k].z >= level, above += v[k].w >= level;
-                if (split - i < 4u) {  // the four with the token: what comes before it in them counts where it is equal
-                    const float u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        for (uint32_t k = 0; k < AT_ONCE; ++k) take2(v[k].x, v[k].y, minus_m), take2(v[k].z, v[k].w, minus_m);
+        if (ranked) {
+            const uint32_t from = head + 4u * j0, to = from + 4u * (AT_ONCE - 1u) * T + 3u;
+            if (to < split || from >= split) {  // all of them on one side of the token
+                const float level = from >= split ? beyond : reach;
 #pragma unroll
-                    for (uint32_t c = 0; c < 4; ++c) above += (int)(u[c] >= (i + c < split ? reach : beyond)) - (int)(u[c] >= level);
+                for (uint32_t k = 0; k < AT_ONCE; ++k) above += v[k].x >= level, above += v[k].y >= level, above += v[k].z >= level, above += v[k].w >= level;
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < AT_ONCE; ++k) {
+                    const uint32_t i = from + 4u * k * T;
+                    above += v[k].x >= (i < split ? reach : beyond), above += v[k].y >= (i + 1u < split ? reach : beyond);
+                    above += v[k].z >= (i + 2u < split ? reach : beyond), above += v[k].w >= (i + 3u < split ? reach : beyond);
                 }
             }
         }
+    };
+    uint32_t j0 = tid;
+    for (; j0 + (AT_ONCE - 1u) * T < fours; j0 += AT_ONCE * T) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = x4[j0 + k * T];
+        take(v, j0);
+    }
+    if (j0 < fours) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = j0 + k * T < fours ? x4[j0 + k * T] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        take(v, j0);
     }
     Sums sums;
     {
         const float2 s = of_pair(s2), t = of_pair(t2);
-        sums = warp_joined(joined(Sums{m, s.x + s.y, t.x + t.y}, Sums{top, 0.0f, 0.0f}));  // its reference is the warp's largest value from here on
+        sums = warp_joined(moved(Sums{m, s.x + s.y, t.x + t.y}, top));  // its reference is the warp's largest value from here on
         uint32_t key = lp_key(top), best = __reduce_max_sync(0xffffffffu, key);
         // the r-th largest of the warp's maxima (equal ones one by one), in warps whose threads all have values, or in the first
         const uint32_t full = max(1u, min(WARPS, fours / 32u)), r = a.top > 1u ? (a.top + full - 1u) / full : 1u;
