@@ -127,49 +127,48 @@ struct Share {
     uint32_t ahead;
     Candidate list[LP_TOP_MAX];
 };
+template <int WARPS>
+struct LpShared {
+    Candidate list[LP_LIST];
+    Sums sums[WARPS];
+    uint32_t ahead[WARPS], reach[WARPS], count, holders;
+    uint16_t holder[32 * WARPS];
+};
 
-// Cluster = one row (one CTA as a rule), CTA c has the values [c * per, (c + 1) * per). The row is read once, with four 16-byte loads of a thread on their way together.
+// A CTA's work on `count` values of a row, from value `first` on.
 //   sums      every thread keeps a reference m, moved only when a value is more than 16 above it, so that exp(x - m) needs no second pass and no rescaling as a
 //             rule; threads, warps and CTAs are joined by (s, t) -> (s e^(m - M), (t + (m - M) s) e^(m - M)). Entropy = log s - t / s.
 //   rank      a value counts where it reaches the token's own, behind the token where it is larger.
-//   list      of k: if every warp has r = ceil(k / warps) threads whose maxima reach a bound, at least k values do, and the k largest are among those. The
-//             least of the warps' r-th largest maxima is such a bound, and few values reach it as a rule; the threads that hold them look at theirs
-//             again (mostly in L1), and they are sorted by counting who comes before whom. Where they are many (equal values, one thread's values above
+//   list      of k: the k-th largest of the warps' maxima (more than the warps: the least of their r-th largest thread maxima, r = ceil(k / warps)) is
+//             reached by at least k values, so the k largest are among those that reach it. These are few as a rule; what the threads hold whose maxima
+//             reach it is looked at again (in L1 or L2), and they are sorted by counting who comes before whom. Where they are many (equal values, one thread's values above
 //             all others), k rounds of a maximum over the block take their place.
-// The CTAs' lists meet in the first one, where a candidate's place is its place in its own list plus what binary search finds in the others.
-// Bound by HBM and the arithmetic on each value for many rows, by a chain of memory and barrier latencies for few.
-template <int T, int CTAS>
-__global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32_t per) {
-    constexpr uint32_t WARPS = T / 32, AT_ONCE = 4;
-    constexpr float SLACK = 16.0f;
-    __shared__ Share s_share[8];
-    __shared__ Candidate s_list[LP_LIST];
-    __shared__ Sums s_sums[WARPS];
-    __shared__ uint32_t s_ahead[WARPS], s_reach[WARPS], s_count;
-    pdl_wait();
-    pdl_trigger();
-    uint32_t peers;
-    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
-    const uint32_t me = tc::cluster_rank(), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const size_t row = blockIdx.x / peers;
-    const float* x = a.logits + row * a.ld + (size_t)me * per;
-    const uint32_t first = me * per, count = min(per, a.n - first);  // first < n
-    if (peers > 1u) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // every CTA of the cluster is there
-    if (tid == 0) s_count = 0u;
-    const uint32_t token = a.tokens ? a.tokens[row] : LP_NONE;
-    const float mine = token < a.n ? clean(a.logits[row * a.ld + token]) : INFINITY;
-    const bool wanted = a.rank && token < a.n, ranked = wanted && mine > -INFINITY && mine < INFINITY;
-    const float reach = ranked ? mine : INFINITY, beyond = ranked ? lp_value(lp_key(mine) + 1u) : INFINITY;
-    const uint32_t here = token - first;  // the token's place among this CTA's values; a token before them is far behind by this count
-    const uint32_t split = token < first ? 0u : here;
-
-    // Values [0, head) and [head + 4 * fours, count) one by one, the others by fours
-    const uint32_t head = min((4u - (uint32_t)(((uintptr_t)x >> 2) & 3u)) & 3u, count), fours = (count - head) / 4u, tail = head + 4u * fours;
-    const float4* x4 = reinterpret_cast<const float4*>(x + head);
+template <int T>
+struct LpRow {
+    static constexpr uint32_t WARPS = T / 32, AT_ONCE = 4;
+    static constexpr float SLACK = 16.0f;
+    const LogprobArgs& a;
+    size_t row;
+    const float* x;
+    const float4* x4;
+    uint32_t tid, first, count, token, split, head, fours, tail;
+    float mine, reach, beyond;
+    bool wanted, ranked;
     float m = -INFINITY, top = -INFINITY;
     uint64_t s2 = 0, t2 = 0;  // two sums each
     uint32_t above = 0;
-    const auto move_to = [&](float largest) {
+
+    __device__ __forceinline__ LpRow(const LogprobArgs& args, size_t r, uint32_t from, uint32_t n, uint32_t tok, float tok_value)
+        : a(args), row(r), tid(threadIdx.x), first(from), count(n), token(tok), mine(tok_value) {
+        x = a.logits + row * a.ld + first;
+        wanted = a.rank && token < a.n, ranked = wanted && mine > -INFINITY && mine < INFINITY;
+        reach = ranked ? mine : INFINITY, beyond = ranked ? lp_value(lp_key(mine) + 1u) : INFINITY;
+        split = token < first ? 0u : token - first;  // the token's place among these values
+        // values [0, head) and [head + 4 * fours, count) one by one, the others by fours
+        head = min((4u - (uint32_t)(((uintptr_t)x >> 2) & 3u)) & 3u, count), fours = (count - head) / 4u, tail = head + 4u * fours;
+        x4 = reinterpret_cast<const float4*>(x + head);
+    }
+    __device__ __forceinline__ void move_to(float largest) {
         if (largest > m + SLACK) {
             const float d = m - largest, e = exp2_fast(d * LP_LOG2E);
             const float2 s = of_pair(s2), t = of_pair(t2);
@@ -177,24 +176,27 @@ __global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32
             s2 = pair_of(s.x * e, s.y * e);
             m = largest;
         }
-    };
-    const auto take2 = [&](float u, float v, uint64_t minus_m) {
+    }
+    __device__ __forceinline__ void take2(float u, float v, uint64_t minus_m) {
         const float2 d = of_pair(add2(pair_of(u, v), minus_m));
         const uint64_t dd = pair_of(fmaxf(d.x, -200.0f), fmaxf(d.y, -200.0f));  // -inf and NaN: 0
         const float2 y = of_pair(mul2(dd, pair_of(LP_LOG2E, LP_LOG2E)));
         const uint64_t e = pair_of(exp2_fast(y.x), exp2_fast(y.y));
         s2 = add2(s2, e);
         t2 = fma2(e, dd, t2);
-    };
-    if (tid < head + (count - tail)) {  // at most six
-        const uint32_t i = tid < head ? tid : tail + tid - head;
-        const float v = clean(x[i]);
-        top = fmaxf(top, v);
-        move_to(v);
-        take2(v, -INFINITY, pair_of(-m, -m));
-        if (ranked) above += v >= (i < split ? reach : beyond);
     }
-    const auto take = [&](const float4 (&v)[AT_ONCE], uint32_t j0) {
+    __device__ __forceinline__ void take_edges() {
+        if (tid < head + (count - tail)) {  // at most six
+            const uint32_t i = tid < head ? tid : tail + tid - head;
+            const float v = clean(x[i]);
+            top = fmaxf(top, v);
+            move_to(v);
+            take2(v, -INFINITY, pair_of(-m, -m));
+            if (ranked) above += v >= (i < split ? reach : beyond);
+        }
+    }
+    // the fours j0, j0 + T, ..
+    __device__ __forceinline__ void take(const float4 (&v)[AT_ONCE], uint32_t j0) {
         float largest = -INFINITY;  // NaN falls out
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; ++k) largest = fmaxf(fmaxf(largest, fmaxf(v[k].x, v[k].y)), fmaxf(v[k].z, v[k].w));
@@ -218,154 +220,209 @@ __global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32
                 }
             }
         }
-    };
-    uint32_t j0 = tid;
-    for (; j0 + (AT_ONCE - 1u) * T < fours; j0 += AT_ONCE * T) {
-        float4 v[AT_ONCE];
-#pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = x4[j0 + k * T];
-        take(v, j0);
     }
-    if (j0 < fours) {
-        float4 v[AT_ONCE];
-#pragma unroll
-        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = j0 + k * T < fours ? x4[j0 + k * T] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        take(v, j0);
-    }
-    Sums sums;
-    {
-        const float2 s = of_pair(s2), t = of_pair(t2);
-        sums = warp_joined(moved(Sums{m, s.x + s.y, t.x + t.y}, top));  // its reference is the warp's largest value from here on
-        uint32_t key = lp_key(top), best = __reduce_max_sync(0xffffffffu, key);
-        // the r-th largest of the warp's maxima (equal ones one by one), in warps whose threads all have values, or in the first
-        const uint32_t full = max(1u, min(WARPS, fours / 32u)), r = a.top > 1u ? (a.top + full - 1u) / full : 1u;
-        for (uint32_t i = 1; i < r; ++i) {
-            const uint32_t holder = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1u;
-            if (lane == holder) key = 0u;
-            best = __reduce_max_sync(0xffffffffu, key);
+    // The CTAs' lists meet in the first one of a cluster, where a candidate's place is its place in its own list plus what binary search finds in the others.
+    __device__ __forceinline__ void finish(LpShared<WARPS>& sh, uint32_t me, uint32_t peers, Share* share) {
+        const uint32_t lane = tid & 31u, warp = tid >> 5;
+        Sums sums;
+        const uint32_t full = max(1u, min(WARPS, fours / 32u));  // warps whose threads all have values, or the first
+        {
+            const float2 s = of_pair(s2), t = of_pair(t2);
+            sums = warp_joined(moved(Sums{m, s.x + s.y, t.x + t.y}, top));  // its reference is the warp's largest value from here on
+            uint32_t key = lp_key(top), best = __reduce_max_sync(0xffffffffu, key);
+            // more alternatives than warps: the r-th largest of the warp's maxima (equal ones one by one)
+            const uint32_t r = (a.top + full - 1u) / full;
+            for (uint32_t i = 1; i < r; ++i) {
+                const uint32_t holder = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1u;
+                if (lane == holder) key = 0u;
+                best = __reduce_max_sync(0xffffffffu, key);
+            }
+            above = __reduce_add_sync(0xffffffffu, above);
+            if (lane == 0) sh.sums[warp] = sums, sh.ahead[warp] = above, sh.reach[warp] = best;
         }
-        above = __reduce_add_sync(0xffffffffu, above);
-        if (lane == 0) s_sums[warp] = sums, s_ahead[warp] = above, s_reach[warp] = warp < full ? best : 0xffffffffu;
-    }
-    __syncthreads();
-    sums = warp_joined(lane < WARPS ? s_sums[lane] : Sums{-INFINITY, 0.0f, 0.0f});
-    above = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_ahead[lane] : 0u);
-    const float bound = a.top > 1u ? lp_value(max(__reduce_min_sync(0xffffffffu, lane < WARPS ? s_reach[lane] : 0xffffffffu), lp_key(-INFINITY))) : sums.m;
-    if (a.top && top >= bound && top > -INFINITY) {
-        const auto meet = [&](uint32_t i, float u) {
-            if (u >= bound && u > -INFINITY) {
-                const uint32_t at = atomicAdd(&s_count, 1u);
-                if (at < LP_LIST) s_list[at] = Candidate{u, first + i};
+        __syncthreads();
+        sums = warp_joined(lane < WARPS ? sh.sums[lane] : Sums{-INFINITY, 0.0f, 0.0f});
+        above = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.ahead[lane] : 0u);
+        float bound = sums.m;
+        if (a.top > 1u) {
+            const uint32_t key = lane < WARPS ? sh.reach[lane] : 0u;
+            uint32_t least = lp_key(-INFINITY);
+            if (a.top <= full) {  // the k-th largest of the warps' maxima, by the upper half of its bits
+                uint32_t prefix = 0u;
+                for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit /= 2u)
+                    if ((uint32_t)__popc(__ballot_sync(0xffffffffu, lane < full && key >= (prefix | bit))) >= a.top) prefix |= bit;
+                least = max(least, prefix);
+            } else {
+                least = max(least, __reduce_min_sync(0xffffffffu, lane < full ? key : 0xffffffffu));
+            }
+            bound = lp_value(least);
+        }
+        if (a.top) {
+            const auto meet = [&](uint32_t i, float u) {
+                if (u >= bound && u > -INFINITY) {
+                    const uint32_t at = atomicAdd(&sh.count, 1u);
+                    if (at < LP_LIST) sh.list[at] = Candidate{u, first + i};
+                }
+            };
+            const auto meet_four = [&](uint32_t j) {
+                const float4 v = x4[j];
+                const uint32_t i = head + 4u * j;
+                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound) meet(i, v.x), meet(i + 1u, v.y), meet(i + 2u, v.z), meet(i + 3u, v.w);
+            };
+            const uint32_t each = (fours + T - 1u) / T;
+            const bool holds = top >= bound && top > -INFINITY;
+            if (holds && tid < head + (count - tail)) {
+                const uint32_t i = tid < head ? tid : tail + tid - head;
+                meet(i, x[i]);
+            }
+            if (each <= 12u) {
+                if (holds)
+#pragma unroll 4
+                    for (uint32_t j = tid; j < fours; j += T) meet_four(j);
+            } else {
+                // many fours a thread: all threads look at the holders' (each at its own, one held up the others for up to 5600 cycles: 64.6 against 54 us for 2048
+                // rows of 32000; with few, the barrier costs more: 32 rows of 131077 18 against 22 us)
+                if (holds) sh.holder[atomicAdd(&sh.holders, 1u)] = (uint16_t)tid;
+                __syncthreads();
+                const uint32_t holders = sh.holders;
+                for (uint32_t w = tid; w < holders * each; w += T) {
+                    const uint32_t q = w / each, j = sh.holder[q] + (w - q * each) * T;
+                    if (j < fours) meet_four(j);
+                }
+            }
+        }
+        // what the sums do not tell: infinities share the probability; the rank of an infinite value is counted value by value
+        const bool infinite = sums.m == INFINITY, recount = wanted && !ranked;
+        if (infinite || recount) {
+            uint32_t n_inf = 0, n_ahead = 0;
+            for (uint32_t i = tid; i < count; i += T) {
+                const float v = clean(x[i]);
+                n_inf += v == INFINITY;
+                n_ahead += v > mine || (v == mine && first + i < token);
+            }
+            n_inf = __reduce_add_sync(0xffffffffu, n_inf);
+            n_ahead = __reduce_add_sync(0xffffffffu, n_ahead);
+            __syncthreads();  // the sums and counts above have been read
+            if (lane == 0) sh.reach[warp] = n_inf, sh.ahead[warp] = n_ahead;
+            __syncthreads();
+            if (infinite) sums.s = (float)__reduce_add_sync(0xffffffffu, lane < WARPS ? sh.reach[lane] : 0u), sums.t = 0.0f;
+            if (recount) above = __reduce_add_sync(0xffffffffu, lane < WARPS ? sh.ahead[lane] : 0u);
+        }
+        __syncthreads();
+        const uint32_t found = sh.count;
+        const bool alone = peers == 1u;
+        const float rest = logf(sums.s);
+        uint32_t remote = 0;  // this CTA's share, in the first one's memory
+        if (alone) {
+            if (tid == 0) lp_store(a, row, sums.m, sums.s, sums.t, token, mine, above);
+        } else {
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            remote = tc::map_to_rank(tc::smem_u32(share + me), 0);
+            if (tid == 0) {
+                tc::st_cluster(remote + offsetof(Share, sums.m), __float_as_uint(sums.m));
+                tc::st_cluster(remote + offsetof(Share, sums.s), __float_as_uint(sums.s));
+                tc::st_cluster(remote + offsetof(Share, sums.t), __float_as_uint(sums.t));
+                tc::st_cluster(remote + offsetof(Share, ahead), above);
+            }
+        }
+        const auto put = [&](uint32_t k, const Candidate& c) {
+            if (alone) {
+                lp_list(a, row, k, c, sums.m, rest);
+            } else {
+                tc::st_cluster(remote + offsetof(Share, list) + k * 8u, __float_as_uint(c.v));
+                tc::st_cluster(remote + offsetof(Share, list) + k * 8u + 4u, c.i);
             }
         };
-        if (tid < head + (count - tail)) {
-            const uint32_t i = tid < head ? tid : tail + tid - head;
-            meet(i, x[i]);
-        }
-#pragma unroll 4
-        for (uint32_t j = tid; j < fours; j += T) {
-            const float4 v = x4[j];
-            const uint32_t i = head + 4u * j;
-            if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= bound) meet(i, v.x), meet(i + 1u, v.y), meet(i + 2u, v.z), meet(i + 3u, v.w);
-        }
-    }
-    // what the sums do not tell: infinities share the probability; the rank of an infinite value is counted value by value
-    const bool infinite = sums.m == INFINITY, recount = wanted && !ranked;
-    if (infinite || recount) {
-        uint32_t n_inf = 0, n_ahead = 0;
-        for (uint32_t i = tid; i < count; i += T) {
-            const float v = clean(x[i]);
-            n_inf += v == INFINITY;
-            n_ahead += v > mine || (v == mine && first + i < token);
-        }
-        n_inf = __reduce_add_sync(0xffffffffu, n_inf);
-        n_ahead = __reduce_add_sync(0xffffffffu, n_ahead);
-        __syncthreads();  // the sums and counts above have been read
-        if (lane == 0) s_reach[warp] = n_inf, s_ahead[warp] = n_ahead;
-        __syncthreads();
-        if (infinite) sums.s = (float)__reduce_add_sync(0xffffffffu, lane < WARPS ? s_reach[lane] : 0u), sums.t = 0.0f;
-        if (recount) above = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_ahead[lane] : 0u);
-    }
-    __syncthreads();
-    const uint32_t found = s_count;
-    const bool alone = peers == 1u;
-    const float rest = logf(sums.s);
-    uint32_t remote = 0;  // this CTA's share, in the first one's memory
-    if (alone) {
-        if (tid == 0) lp_store(a, row, sums.m, sums.s, sums.t, token, mine, above);
-    } else {
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-        remote = tc::map_to_rank(tc::smem_u32(s_share + me), 0);
-        if (tid == 0) {
-            tc::st_cluster(remote + offsetof(Share, sums.m), __float_as_uint(sums.m));
-            tc::st_cluster(remote + offsetof(Share, sums.s), __float_as_uint(sums.s));
-            tc::st_cluster(remote + offsetof(Share, sums.t), __float_as_uint(sums.t));
-            tc::st_cluster(remote + offsetof(Share, ahead), above);
-        }
-    }
-    const auto put = [&](uint32_t k, const Candidate& c) {
-        if (alone) {
-            lp_list(a, row, k, c, sums.m, rest);
-        } else {
-            tc::st_cluster(remote + offsetof(Share, list) + k * 8u, __float_as_uint(c.v));
-            tc::st_cluster(remote + offsetof(Share, list) + k * 8u + 4u, c.i);
-        }
-    };
-    if (found <= LP_LIST) {
-        // four threads count for one candidate
-        for (uint32_t c = tid / 4u; c < ((found + 7u) & ~7u); c += T / 4u) {
-            const Candidate own = s_list[min(c, LP_LIST - 1u)];
-            uint32_t place = 0;
-            for (uint32_t j = tid & 3u; j < found; j += 4u) place += before(s_list[j], own);
-            place += __shfl_xor_sync(0xffffffffu, place, 1);
-            place += __shfl_xor_sync(0xffffffffu, place, 2);
-            if ((tid & 3u) == 0 && c < found && place < a.top) put(place, own);
-        }
-        for (uint32_t k = found + tid; k < a.top; k += T) put(k, Candidate{-INFINITY, LP_NONE});
-    } else {
-        Candidate prev = {INFINITY, 0u};
-        for (uint32_t r = 0; r < a.top; ++r) {
-            Candidate best = {-INFINITY, LP_NONE};
-            for (uint32_t i = tid; i < count; i += T) {
-                const Candidate c = {clean(x[i]), first + i};
-                if (c.v > -INFINITY && (r == 0 || before(prev, c)) && before(c, best)) best = c;
+        if (found <= LP_LIST) {
+            // four threads count for one candidate
+            for (uint32_t c = tid / 4u; c < ((found + 7u) & ~7u); c += T / 4u) {
+                const Candidate own = sh.list[min(c, LP_LIST - 1u)];
+                uint32_t place = 0;
+                for (uint32_t j = tid & 3u; j < found; j += 4u) place += before(sh.list[j], own);
+                place += __shfl_xor_sync(0xffffffffu, place, 1);
+                place += __shfl_xor_sync(0xffffffffu, place, 2);
+                if ((tid & 3u) == 0 && c < found && place < a.top) put(place, own);
             }
-            best = warp_best(best);
-            __syncthreads();
-            if (lane == 0) s_list[warp] = best;
-            __syncthreads();
-            best = warp_best(lane < WARPS ? s_list[lane] : Candidate{-INFINITY, LP_NONE});
-            if (tid == 0) put(r, best);
-            prev = best;
+            for (uint32_t k = found + tid; k < a.top; k += T) put(k, Candidate{-INFINITY, LP_NONE});
+        } else {
+            Candidate prev = {INFINITY, 0u};
+            for (uint32_t r = 0; r < a.top; ++r) {
+                Candidate best = {-INFINITY, LP_NONE};
+                for (uint32_t i = tid; i < count; i += T) {
+                    const Candidate c = {clean(x[i]), first + i};
+                    if (c.v > -INFINITY && (r == 0 || before(prev, c)) && before(c, best)) best = c;
+                }
+                best = warp_best(best);
+                __syncthreads();
+                if (lane == 0) sh.list[warp] = best;
+                __syncthreads();
+                best = warp_best(lane < WARPS ? sh.list[lane] : Candidate{-INFINITY, LP_NONE});
+                if (tid == 0) put(r, best);
+                prev = best;
+            }
+        }
+        if (alone) return;
+        tc::cluster_sync_all();
+        if (me != 0) return;
+
+        sums = warp_joined(lane < peers ? share[lane].sums : Sums{-INFINITY, 0.0f, 0.0f});
+        above = __reduce_add_sync(0xffffffffu, lane < peers ? share[lane].ahead : 0u);
+        if (tid == 0) lp_store(a, row, sums.m, sums.s, sums.t, token, mine, above);
+        const float rest_all = logf(sums.s);
+        for (uint32_t q = tid; q < peers * a.top; q += T) {
+            const uint32_t c = q / a.top, k = q - c * a.top;
+            const Candidate own = share[c].list[k];
+            uint32_t lo[8], place = k;  // the values of the other lists that come before this one; the lists' empty places end them
+#pragma unroll
+            for (uint32_t o = 0; o < 8u; ++o) lo[o] = 0;
+            const bool empty = own.i == LP_NONE;
+            for (uint32_t step = 64u; step; step /= 2u)
+#pragma unroll
+                for (uint32_t o = 0; o < 8u; ++o)
+                    if (o < peers && lo[o] + step <= a.top) {
+                        const Candidate u = share[o].list[lo[o] + step - 1u];
+                        if (u.i != LP_NONE && (empty || before(u, own))) lo[o] += step;
+                    }
+#pragma unroll
+            for (uint32_t o = 0; o < 8u; ++o)  // an empty place comes behind every value and behind the empty places of the lists before its own
+                if (o < peers && o != c) place += empty && o < c ? a.top : lo[o];
+            if (place < a.top) lp_list(a, row, place, own, sums.m, rest_all);
         }
     }
-    if (alone) return;
-    tc::cluster_sync_all();
-    if (me != 0) return;
+};
 
-    sums = warp_joined(lane < peers ? s_share[lane].sums : Sums{-INFINITY, 0.0f, 0.0f});
-    above = __reduce_add_sync(0xffffffffu, lane < peers ? s_share[lane].ahead : 0u);
-    if (tid == 0) lp_store(a, row, sums.m, sums.s, sums.t, token, mine, above);
-    const float rest_all = logf(sums.s);
-    for (uint32_t q = tid; q < peers * a.top; q += T) {
-        const uint32_t c = q / a.top, k = q - c * a.top;
-        const Candidate own = s_share[c].list[k];
-        uint32_t lo[8], place = k;  // the values of the other lists that come before this one; the lists' empty places end them
+// Cluster = one row (one CTA as a rule), CTA c has the values [c * per, (c + 1) * per). The row is read once, with four 16-byte loads of a thread on their way
+// together. Bound by a chain of memory and barrier latencies.
+template <int T, int CTAS>
+__global__ void __launch_bounds__(T, CTAS) logprobs_kernel(LogprobArgs a, uint32_t per) {
+    __shared__ Share s_share[8];
+    __shared__ LpShared<T / 32> sh;
+    pdl_wait();
+    pdl_trigger();
+    uint32_t peers;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
+    const uint32_t me = tc::cluster_rank(), tid = threadIdx.x, first = me * per;  // first < n
+    const size_t row = blockIdx.x / peers;
+    if (peers > 1u) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // every CTA of the cluster is there
+    if (tid == 0) sh.count = 0u, sh.holders = 0u;
+    const uint32_t token = a.tokens ? a.tokens[row] : LP_NONE;
+    LpRow<T> r(a, row, first, min(per, a.n - first), token, token < a.n ? clean(a.logits[row * a.ld + token]) : INFINITY);
+    r.take_edges();
+    constexpr uint32_t AT_ONCE = LpRow<T>::AT_ONCE;
+    uint32_t j0 = tid;
+    for (; j0 + (AT_ONCE - 1u) * T < r.fours; j0 += AT_ONCE * T) {
+        float4 v[AT_ONCE];
 #pragma unroll
-        for (uint32_t o = 0; o < 8u; ++o) lo[o] = 0;
-        const bool empty = own.i == LP_NONE;
-        for (uint32_t step = 64u; step; step /= 2u)
-#pragma unroll
-            for (uint32_t o = 0; o < 8u; ++o)
-                if (o < peers && lo[o] + step <= a.top) {
-                    const Candidate u = s_share[o].list[lo[o] + step - 1u];
-                    if (u.i != LP_NONE && (empty || before(u, own))) lo[o] += step;
-                }
-#pragma unroll
-        for (uint32_t o = 0; o < 8u; ++o)  // an empty place comes behind every value and behind the empty places of the lists before its own
-            if (o < peers && o != c) place += empty && o < c ? a.top : lo[o];
-        if (place < a.top) lp_list(a, row, place, own, sums.m, rest_all);
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = r.x4[j0 + k * T];
+        r.take(v, j0);
     }
+    if (j0 < r.fours) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (uint32_t k = 0; k < AT_ONCE; ++k) v[k] = j0 + k * T < r.fours ? r.x4[j0 + k * T] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        r.take(v, j0);
+    }
+    r.finish(sh, me, peers, s_share);
 }
 
 template <int T, int CTAS>

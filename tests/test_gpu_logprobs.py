@@ -73,12 +73,14 @@ def test_sizes(nat, n, rows, top):
     assert got["rank"][0] == 1 and T.status(nat) == 0
 
 
-@pytest.mark.parametrize("rows", [7, 64, 149, 400])
-def test_many_rows(nat, rows):
+@pytest.mark.parametrize("rows,n,ld", [(7, 2003, 0), (64, 2003, 0), (149, 2003, 0), (400, 2003, 0), (445, 2003, 0), (1000, 2003, 0), (900, 1, 0), (700, 6, 0),
+                                       (500, 4095, 4101), (500, 4096, 0), (460, 9001, 0), (889, 1000, 1001)])
+def test_many_rows(nat, rows, n, ld):
     rng = np.random.default_rng(rows)
-    x = (4 * rng.standard_normal((rows, 2003))).astype(np.float32)
-    tokens = rng.integers(0, 2003, rows)
-    check(x, tokens, 7, run(nat, x, tokens, 7))
+    x = (4 * rng.standard_normal((rows, n))).astype(np.float32)
+    tokens = rng.integers(0, n, rows)
+    check(x, tokens, 7, run(nat, x, tokens, 7, ld=ld))
+    assert T.status(nat) == 0
 
 
 @pytest.mark.parametrize("ld", [0, 5003, 5004, 5120])
@@ -91,8 +93,8 @@ def test_pitch(nat, ld):
 
 @pytest.mark.parametrize("name", ["equal", "few values", "ascending", "descending", "one large", "close", "masked", "nan", "infinite", "all masked", "all nan",
                                   "few left", "one thread's", "far apart", "huge"])
-@pytest.mark.parametrize("n", [600, 33000])
-def test_rows_of_every_kind(nat, name, n):
+@pytest.mark.parametrize("n,times", [(600, 1), (33000, 1), (9001, 150)])
+def test_rows_of_every_kind(nat, name, n, times):
     rng = np.random.default_rng(len(name))
     x = (3 * rng.standard_normal((3, n))).astype(np.float32)
     if name == "equal":
@@ -130,7 +132,14 @@ def test_rows_of_every_kind(nat, name, n):
     elif name == "huge":
         x = (np.finfo(np.float32).max * rng.uniform(-1, 1, x.shape)).astype(np.float32)
     tokens = np.array([5, n - 1, 7])
-    check(x, tokens, 20, run(nat, x, tokens, 20))
+    if times == 1:
+        check(x, tokens, 20, run(nat, x, tokens, 20))
+        return
+    got = run(nat, np.tile(x, (times, 1)), np.tile(tokens, times), 20)  # a long batch of the three rows
+    for at in range(0, 12, 3):
+        check(x, tokens, 20, {k: v[at:at + 3] for k, v in got.items()})
+    for k, v in got.items():  # a row's place within 16 bytes decides which thread adds which value: it comes back after 12 rows, and with it every bit
+        assert all(np.array_equal(v[i - 12], v[i]) for i in range(12, 3 * times)), k
 
 
 def test_outputs_may_be_left_out(nat):
