@@ -452,14 +452,16 @@ extern "C" int m40llm_logprobs_f32_async(M40llmCudaContext* ctx, const M40llmLog
     const LogprobArgs a = {(const float*)c->logits, c->tokens, (float*)c->logprob, c->rank, (float*)c->entropy, (float*)c->lse, c->top_ids,
                            (float*)c->top_logprobs, ctx->d_status, c->n, c->ld ? c->ld : c->n,
                            c->top_ids || c->top_logprobs ? c->top : 0u};
-    // Many rows: a CTA of 512 threads each (2048 rows of 32000 values 68 us; 73 with 256, 85 with 1024). Few: 1024 threads, and up to 8 CTAs that have 32768
-    // values (a row of 32000: one CTA 10.0 us, two 11.2, four 12.5).
-    const bool few = 2ull * c->rows <= (uint64_t)ctx->sm_count;
+    // More rows than SMs: a CTA of 256 threads each, five per SM (2048 rows of 32000 values 50.4 us, 300 rows 14.2; with 512 threads 54.7 and 14.6, with 128
+    // and twice the loads 48.6 and 19.6). Else 1024 threads (80 rows 7.3 us against 8.5), and up to 8 CTAs that have 32768 values or more (a row of 32000: one
+    // CTA 10.0 us, two 11.2, four 12.5).
+    const uint64_t sms = (uint64_t)ctx->sm_count;
     uint32_t peers = 1u;
-    while (few && peers < 8u && (uint64_t)peers * 2u * c->rows <= (uint64_t)ctx->sm_count && c->n > 32768u * peers) peers *= 2u;
+    while (peers < 8u && peers * 2ull * c->rows <= sms && c->n > 32768u * peers) peers *= 2u;
     const uint32_t per = (((c->n + peers - 1u) / peers) + 3u) & ~3u;
     peers = (c->n + per - 1u) / per;  // no CTA without values
-    const cudaError_t e = few ? launch_logprobs<1024, 1>(a, c->rows, peers, per, ctx->decode_stream) : launch_logprobs<512, 3>(a, c->rows, peers, per, ctx->decode_stream);
+    const cudaError_t e = c->rows <= sms ? launch_logprobs<1024, 1>(a, c->rows, peers, per, ctx->decode_stream)
+                                         : launch_logprobs<256, 5>(a, c->rows, peers, per, ctx->decode_stream);
     M40_COUNT_LAUNCH(ctx);
     if (e != cudaSuccess) {
         cudaGetLastError();
