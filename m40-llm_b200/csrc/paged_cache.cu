@@ -1,6 +1,7 @@
 // A key / value cache in pages: append (with rotation) and eviction by accumulated attention weight.
 #include "paged.cuh"
 #include "stack_math.cuh"
+#include "tc_ptx.cuh"
 
 namespace {
 
@@ -86,15 +87,18 @@ struct EvictArgs {
     float* weights_out;
     const uint32_t* entry_pos;
     uint32_t* entry_pos_out;
-    uint32_t* origin;   // [count][kv_heads][keep]
+    uint32_t* origin;   // [count][kv_heads][keep] or null
     uint32_t* new_len;  // [count]
-    uint32_t* holes;    // scratch [count][kv_heads][keep]: free places below the new end
-    uint32_t* late;     // scratch, likewise: kept entries behind it
+    uint32_t* plan;     // scratch [count][kv_heads][keep]: a place's own entry, EVICT_HOLE + the hole's number, or PAGED_NONE beyond the new length
+    uint32_t* late;     // scratch, likewise: kept entries behind the new end, in order
     uint32_t* status;
     uint32_t keep, first, recent, ld, bound, in_place;
+    uint32_t cached;    // entries that a CTA's shared memory holds
 };
 
-constexpr uint32_t SELECT_THREADS = 1024;
+constexpr uint32_t SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, EVICT_HOLE = 0x80000000u, SELECT_CLUSTER = 8;
+constexpr uint32_t SELECT_CACHED = 24576;  // entries with key and position in 192 KB
+constexpr int SELECT_BITS = 11, SELECT_BINS = 1 << SELECT_BITS, SELECT_PASSES = 3;  // 32 bits in 11, 11 and 10
 
 // Larger is better. Held entries come before every weight (+inf is 0xff800000), NaN after every other.
 __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
@@ -104,146 +108,285 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// Sum of x over the threads before this one; `total` gets the block's. Two barriers.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warps, uint32_t* total) {
+// Sum over the warps before this one of a value per warp, and over all of them; `warps` is shared memory for SELECT_WARPS values. Two barriers.
+__device__ __forceinline__ uint4 warps_before(const uint4& mine, uint4* warps, uint4* total) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    uint32_t v = x;
+    __syncthreads();
+    if (lane == 0) warps[warp] = mine;
+    __syncthreads();
+    const uint4 x = warps[lane];  // SELECT_WARPS is 32
+    const auto upto = [&](uint32_t v, uint32_t* all) {
+        uint32_t sum = v;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= (uint32_t)o) v += u;
-    }
-    __syncthreads();
-    if (lane == 31u) warps[warp] = v;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (uint32_t w = 0; w < SELECT_THREADS / 32; ++w) {
-        if (w < warp) before += warps[w];
-        all += warps[w];
-    }
-    *total = all;
-    return before + v - x;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= (uint32_t)o) sum += u;
+        }
+        *all = __shfl_sync(0xffffffffu, sum, 31);
+        return __shfl_sync(0xffffffffu, sum - v, warp);
+    };
+    uint4 r;
+    r.x = upto(x.x, &total->x), r.y = upto(x.y, &total->y), r.z = upto(x.z, &total->z), r.w = upto(x.w, &total->w);
+    return r;
 }
 
-// CTA = (listed sequence, kv head). The key of the last kept entry is found by its bytes, from the highest down (256 bins each); one more pass over
-// the entries in order deals the ties, and notes the holes below the new end and the kept entries behind it.
+struct SelectShared {
+    uint32_t bins[SELECT_PASSES][SELECT_BINS];  // one set per pass: a pass needs no barrier after its counts were read
+    uint4 warps[SELECT_WARPS];
+    uint4 counts;                               // this CTA's: larger and equal keys below the new end, then behind it
+    uint32_t newest, pick[2];
+};
+
+// Cluster of CTAs = (listed sequence, kv head); a CTA has a run of its entries, their keys in shared memory where they fit (else they are made again in every
+// pass). The key of the last kept entry is found by its bits from the highest down: a histogram per CTA, summed up through distributed shared memory, in every
+// CTA alike. Then the entries are counted once, larger and equal ones below and behind the new end, which gives every warp the numbers of its ties,
+// holes and kept entries behind the end, so that the plan is written without an order of who comes first. Against one CTA and four passes from memory: 4 x 8
+// heads of 8192 entries 68 -> @E us, 8 heads of 32768 200 -> @F. Bound by the barriers of the cluster.
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t bins[256], warps[SELECT_THREADS / 32], s_pick[2], s_end;
+    extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions
+    __shared__ SelectShared sh;
+    uint32_t peers;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
+    const uint32_t me = tc::cluster_rank(), h = blockIdx.x / peers, i = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    for (uint32_t b = tid; b < SELECT_PASSES * SELECT_BINS; b += SELECT_THREADS) (&sh.bins[0][0])[b] = 0u;
+    if (tid == 0) sh.newest = 0u;
     pdl_wait();
     pdl_trigger();
-    const uint32_t i = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
     const uint32_t slot = a.seq[i], len = a.len[i];
-    bool bad = slot >= a.c.slots || len > a.bound;
-    if (tid == 0) s_end = 0u;
     int twice = 0;
     for (uint32_t j = tid; j < i; j += SELECT_THREADS) twice |= a.seq[j] == slot;
-    if (__syncthreads_or(twice)) bad = true;
-    uint32_t* from = a.origin + ((size_t)i * a.c.kv_heads + h) * a.keep;
+    const bool bad = __syncthreads_or(twice) || slot >= a.c.slots || len > a.bound;  // the same in every CTA of the cluster
+    uint32_t* plan = a.plan + ((size_t)i * a.c.kv_heads + h) * a.keep;
     const uint32_t kept = bad ? 0u : min(len, a.keep);
-    if (tid == 0 && h == 0) {
+    if (tid == 0 && h == 0 && me == 0) {
         a.new_len[i] = kept;
         if (bad) atomicOr(a.status, 1u);
     }
-    for (uint32_t e = kept + tid; e < a.keep; e += SELECT_THREADS) from[e] = PAGED_NONE;
+    const uint32_t all = me * SELECT_THREADS + tid, step = peers * SELECT_THREADS;
+    for (uint32_t e = kept + all; e < a.keep; e += step) plan[e] = PAGED_NONE;
     if (kept == 0 || len <= a.keep) {
-        for (uint32_t e = tid; e < kept; e += SELECT_THREADS) from[e] = e;
+        for (uint32_t e = all; e < kept; e += step) plan[e] = e;
         return;
     }
     const size_t base = ((size_t)slot * a.c.kv_heads + h) * a.ld;
     const float* w = a.weights + base;
     const uint32_t* pos = a.entry_pos ? a.entry_pos + base : nullptr;
+    // this CTA's entries [lo, hi), and in them the warp's [wlo, whi)
+    const uint32_t per = (len + peers - 1u) / peers, lo = min(me * per, len), hi = min(lo + per, len), mine = hi - lo;
+    const uint32_t per_warp = ((per + SELECT_WARPS - 1u) / SELECT_WARPS + 31u) & ~31u, wlo = min(lo + warp * per_warp, hi), whi = min(wlo + per_warp, hi);
+    const bool cached = per <= a.cached;
+    uint32_t* s_key = s_dyn;
+    uint32_t* s_pos = s_dyn + a.cached;
     uint32_t newest = 0;
-    if (pos)
-        for (uint32_t e = tid; e < len; e += SELECT_THREADS) newest = max(newest, pos[e]);
-    else
+    if (pos) {
+#pragma unroll 4
+        for (uint32_t j = tid; j < mine; j += SELECT_THREADS) {
+            const uint32_t p = pos[lo + j];
+            if (cached) s_pos[j] = p, s_key[j] = evict_key(w[lo + j], false);
+            newest = max(newest, p);
+        }
+        newest = __reduce_max_sync(0xffffffffu, newest);
+        if (lane == 0) atomicMax(&sh.newest, newest);
+        __syncthreads();
+        tc::cluster_sync_all();
+        newest = lane < peers ? tc::ld_cluster(tc::map_to_rank(tc::smem_u32(&sh.newest), lane)) : 0u;
+        newest = __reduce_max_sync(0xffffffffu, newest);
+    } else {
         newest = len - 1u;
-    newest = __reduce_max_sync(0xffffffffu, newest);
-    if ((tid & 31u) == 0) atomicMax(&s_end, newest);
-    __syncthreads();
-    newest = s_end;
-    auto key = [&](uint32_t e) {
+    }
+    const auto fresh = [&](uint32_t e) {
         const uint32_t p = pos ? pos[e] : e;
         return evict_key(w[e], p < a.first || newest - p < a.recent);
     };
+    if (cached)
+        for (uint32_t j = tid; j < mine; j += SELECT_THREADS) {
+            if (!pos) {
+                s_key[j] = fresh(lo + j);
+            } else {
+                const uint32_t p = s_pos[j];
+                if (p < a.first || newest - p < a.recent) s_key[j] = 0xffffffffu;
+            }
+        }
+    const auto key = [&](uint32_t e) { return cached ? s_key[e - lo] : fresh(e); };
+
     uint32_t prefix = 0, want = a.keep;  // the want-th largest among the keys that begin with prefix
-    for (int byte = 3; byte >= 0; --byte) {
-        const uint32_t high = byte == 3 ? 0u : 0xffffffffu << (8 * (byte + 1));
-        for (uint32_t b = tid; b < 256u; b += SELECT_THREADS) bins[b] = 0;
-        __syncthreads();
-        for (uint32_t e = tid; e < len; e += SELECT_THREADS) {
-            const uint32_t k = key(e);
-            if ((k & high) == prefix) atomicAdd(&bins[(k >> (8 * byte)) & 255u], 1u);
+#pragma unroll
+    for (int pass = 0; pass < SELECT_PASSES; ++pass) {
+        const int shift = pass == 0 ? 32 - SELECT_BITS : (pass == 1 ? 32 - 2 * SELECT_BITS : 0), bits = pass == 2 ? 32 - 2 * SELECT_BITS : SELECT_BITS;
+        const uint32_t high = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
+        uint32_t* bins = sh.bins[pass];
+        // the thread's own keys: it made them. Lanes that meet in a bin add once.
+        for (uint32_t j0 = 0; j0 < mine; j0 += SELECT_THREADS) {
+            const uint32_t j = j0 + tid;
+            const uint32_t k = j < mine ? key(lo + j) : 0u;
+            const bool in = j < mine && (k & high) == prefix;
+            const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
+            const uint32_t same = __match_any_sync(0xffffffffu, in ? bin : 0xffffffffu);
+            if (in && (same & ((1u << lane) - 1u)) == 0u) atomicAdd(&bins[bin], (uint32_t)__popc(same));
         }
         __syncthreads();
-        if (tid == 0) {
-            uint32_t b = 255u, above = 0;
-            while (above + bins[b] < want) above += bins[b--];
-            s_pick[0] = b;
-            s_pick[1] = want - above;
+        if (peers > 1u) tc::cluster_sync_all();
+        // thread t: the bins from the top, 2 t and 2 t + 1
+        constexpr uint32_t top = SELECT_BINS - 1;
+        uint32_t n0 = 0, n1 = 0;
+        const uint32_t at = tc::smem_u32(bins + (top - 2u * tid - 1u));
+#pragma unroll
+        for (uint32_t c = 0; c < SELECT_CLUSTER; ++c)
+            if (c < peers) {
+                const uint2 n = tc::ld_cluster2(tc::map_to_rank(at, c));
+                n0 += n.y, n1 += n.x;
+            }
+        uint32_t sum = n0 + n1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= (uint32_t)o) sum += u;
+        }
+        if (lane == 31u) sh.warps[warp].x = sum;
+        __syncthreads();
+        uint32_t above = lane < warp ? sh.warps[lane].x : 0u;
+        above = __reduce_add_sync(0xffffffffu, above) + sum - n0 - n1;  // entries in the bins above this thread's
+        if (above < want && above + n0 + n1 >= want) {
+            const bool upper = above + n0 >= want;
+            sh.pick[0] = top - 2u * tid - (upper ? 0u : 1u);
+            sh.pick[1] = want - above - (upper ? 0u : n0);
         }
         __syncthreads();
-        prefix |= s_pick[0] << (8 * byte);
-        want = s_pick[1];
-        __syncthreads();
+        prefix |= sh.pick[0] << shift;
+        want = sh.pick[1];
     }
-    uint32_t* holes = a.holes + ((size_t)i * a.c.kv_heads + h) * a.keep;
-    uint32_t* late = a.late + ((size_t)i * a.c.kv_heads + h) * a.keep;
-    uint32_t ties = 0, n_holes = 0, n_late = 0;
-    for (uint32_t e0 = 0; e0 < len; e0 += SELECT_THREADS) {
-        const uint32_t e = e0 + tid;
-        const uint32_t k = e < len ? key(e) : 0u;
-        const bool tie = e < len && k == prefix;
-        uint32_t total;
-        const uint32_t rank = ties + block_scan(tie ? 1u : 0u, warps, &total);
-        ties += total;
-        const bool stays = e < len && (k > prefix || (tie && rank < want));
-        const bool hole = e < a.keep && !stays, behind = e >= a.keep && stays;
-        const uint32_t nh = n_holes + block_scan(hole ? 1u : 0u, warps, &total);
-        n_holes += total;
-        const uint32_t nl = n_late + block_scan(behind ? 1u : 0u, warps, &total);
-        n_late += total;
-        if (stays && e < a.keep) from[e] = e;
-        if (hole) holes[nh] = e;
-        if (behind) late[nl] = e;
+
+    uint4 count = make_uint4(0, 0, 0, 0);  // larger, equal below the new end; larger, equal behind it
+    for (uint32_t e0 = wlo; e0 < whi; e0 += 32u) {
+        const uint32_t e = e0 + lane, k = e < whi ? key(e) : 0u;
+        const bool larger = e < whi && k > prefix, equal = e < whi && k == prefix, below = e < a.keep;
+        count.x += __popc(__ballot_sync(0xffffffffu, larger && below)), count.y += __popc(__ballot_sync(0xffffffffu, equal && below));
+        count.z += __popc(__ballot_sync(0xffffffffu, larger && !below)), count.w += __popc(__ballot_sync(0xffffffffu, equal && !below));
     }
+    uint4 total;
+    uint4 before = warps_before(count, sh.warps, &total);
+    if (tid == 0) sh.counts = total;
     __syncthreads();
-    for (uint32_t j = tid; j < n_holes; j += SELECT_THREADS) from[holes[j]] = late[j];
+    if (peers > 1u) {
+        tc::cluster_sync_all();
+        uint4 other = make_uint4(0, 0, 0, 0);
+        if (lane < me) {
+            const uint32_t from = tc::map_to_rank(tc::smem_u32(&sh.counts), lane);
+            other = make_uint4(tc::ld_cluster(from), tc::ld_cluster(from + 4u), tc::ld_cluster(from + 8u), tc::ld_cluster(from + 12u));
+        }
+        before.x += __reduce_add_sync(0xffffffffu, other.x), before.y += __reduce_add_sync(0xffffffffu, other.y);
+        before.z += __reduce_add_sync(0xffffffffu, other.z), before.w += __reduce_add_sync(0xffffffffu, other.w);
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read what it needs of the others
+    }
+    // Entries below the end come before those behind it, so the ties, kept entries and holes before the warp follow from the four counts. As the first
+    // `want` ties stay: below the end, kept = larger + min(ties, want).
+    uint32_t ties = before.y + before.w, holes, late;
+    {
+        const uint32_t entries_below = min(wlo, a.keep);
+        holes = entries_below - (before.x + min(before.y, want));
+        const uint32_t ties_behind = before.w;  // only where the warp's entries begin behind the end are these counted, and then all ties below are before them
+        late = before.z + (min(before.y + ties_behind, want) - min(before.y, want));
+    }
+    uint32_t* late_list = a.late + ((size_t)i * a.c.kv_heads + h) * a.keep;
+    const uint32_t under = (1u << lane) - 1u;
+    for (uint32_t e0 = wlo; e0 < whi; e0 += 32u) {
+        const uint32_t e = e0 + lane, k = e < whi ? key(e) : 0u;
+        const bool equal = e < whi && k == prefix, below = e < a.keep;
+        const uint32_t tie_mask = __ballot_sync(0xffffffffu, equal);
+        const bool stays = e < whi && (k > prefix || (equal && ties + __popc(tie_mask & under) < want));
+        ties += __popc(tie_mask);
+        const bool hole = e < whi && below && !stays, behind = stays && !below;
+        const uint32_t hole_mask = __ballot_sync(0xffffffffu, hole), late_mask = __ballot_sync(0xffffffffu, behind);
+        if (e < whi && below) plan[e] = stays ? e : EVICT_HOLE + holes + __popc(hole_mask & under);
+        if (behind) late_list[late + __popc(late_mask & under)] = e;
+        holes += __popc(hole_mask);
+        late += __popc(late_mask);
+    }
+    if (peers > 1u) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its counts are read
 }
 
-// Warp = one kept place of one kv head. In place a source lies behind the new end and a target before it, so that no copy reads what
-// another writes.
+// Warp = MOVE_PLACES kept places of one kv head, their loads on their way together. In place a source lies behind the new end and a target before it, so
+// that no copy reads what another writes. Bound by HBM and the chain plan, late list, page tables, rows.
+constexpr uint32_t MOVE_PLACES = 4;
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t row_bytes, uint32_t elem, uint32_t vec) {
     pdl_wait();
     pdl_trigger();
-    const uint32_t i = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31u, place = blockIdx.x * 8u + (threadIdx.x >> 5);
-    if (place >= a.keep) return;
-    const uint32_t src = a.origin[((size_t)i * a.c.kv_heads + h) * a.keep + place];
-    if (src == PAGED_NONE) return;
+    const uint32_t i = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31u, place0 = (blockIdx.x * 8u + (threadIdx.x >> 5)) * MOVE_PLACES;
+    if (place0 >= a.keep) return;
     const uint32_t slot = a.seq[i];
-    const size_t base = ((size_t)slot * a.c.kv_heads + h) * a.ld;
-    if (lane == 0) {
-        if (a.weights_out && (src != place || a.weights_out != a.weights)) a.weights_out[base + place] = a.weights[base + src];
-        if (a.entry_pos_out && (src != place || a.entry_pos_out != a.entry_pos)) a.entry_pos_out[base + place] = a.entry_pos ? a.entry_pos[base + src] : src;
+    const size_t list = ((size_t)i * a.c.kv_heads + h) * a.keep, base = ((size_t)slot * a.c.kv_heads + h) * a.ld;
+    // lanes 0 .. MOVE_PLACES - 1 look a place up each
+    uint32_t src = PAGED_NONE, from = PAGED_NONE, into = PAGED_NONE;
+    const uint32_t place = place0 + lane;
+    if (lane < MOVE_PLACES && place < a.keep) {
+        src = a.plan[list + place];
+        if (src != PAGED_NONE && src >= EVICT_HOLE) src = a.late[list + (src - EVICT_HOLE)];
+        if (a.origin) a.origin[list + place] = src;
+        if (src != PAGED_NONE) {
+            const bool stays_put = a.in_place && src == place;
+            if (!stays_put) {
+                from = paged_page(a.c, slot, src), into = paged_page(a.to, slot, place);
+                if (from == PAGED_NONE || into == PAGED_NONE) {
+                    atomicOr(a.status, from == PAGED_NONE ? 1u : 2u);
+                    from = PAGED_NONE;
+                }
+            }
+            if (a.weights_out && (src != place || a.weights_out != a.weights)) a.weights_out[base + place] = a.weights[base + src];
+            if (a.entry_pos_out && (src != place || a.entry_pos_out != a.entry_pos)) a.entry_pos_out[base + place] = a.entry_pos ? a.entry_pos[base + src] : src;
+        }
     }
-    if (a.in_place && src == place) return;
-    const uint32_t from = paged_page(a.c, slot, src), into = paged_page(a.to, slot, place);
-    if (from == PAGED_NONE || into == PAGED_NONE) {
-        if (lane == 0) atomicOr(a.status, from == PAGED_NONE ? 1u : 2u);
-        return;
+    size_t s[MOVE_PLACES], d[MOVE_PLACES];
+    bool moves[MOVE_PLACES];
+#pragma unroll
+    for (uint32_t k = 0; k < MOVE_PLACES; ++k) {
+        const uint32_t f = __shfl_sync(0xffffffffu, from, k), t = __shfl_sync(0xffffffffu, into, k), e = __shfl_sync(0xffffffffu, src, k);
+        moves[k] = f != PAGED_NONE;
+        s[k] = moves[k] ? paged_row(a.c, f, h, e) * elem : 0;
+        d[k] = moves[k] ? paged_row(a.to, t, h, place0 + k) * elem : 0;
     }
-    const size_t s = paged_row(a.c, from, h, src) * elem, d = paged_row(a.to, into, h, place) * elem;
     if (vec) {
-        for (uint32_t b = lane * 16u; b < row_bytes; b += 512u) {
-            const uint4 x = *reinterpret_cast<const uint4*>(a.c.k + s + b), y = *reinterpret_cast<const uint4*>(a.c.v + s + b);
-            *reinterpret_cast<uint4*>(a.to.k + d + b) = x;
-            *reinterpret_cast<uint4*>(a.to.v + d + b) = y;
+        // 16-byte pieces of a key row, then of its value row
+        const uint32_t half = row_bytes / 16u;
+        for (uint32_t p = lane; p < 2u * half; p += 32u) {
+            const bool value = p >= half;
+            const uint32_t b = (value ? p - half : p) * 16u;
+            const unsigned char* in = value ? a.c.v : a.c.k;
+            unsigned char* out = value ? a.to.v : a.to.k;
+            uint4 x[MOVE_PLACES];
+#pragma unroll
+            for (uint32_t k = 0; k < MOVE_PLACES; ++k)
+                if (moves[k]) x[k] = *reinterpret_cast<const uint4*>(in + s[k] + b);
+#pragma unroll
+            for (uint32_t k = 0; k < MOVE_PLACES; ++k)
+                if (moves[k]) *reinterpret_cast<uint4*>(out + d[k] + b) = x[k];
         }
     } else {
-        for (uint32_t b = lane * 2u; b < row_bytes; b += 64u) {
-            *reinterpret_cast<uint16_t*>(a.to.k + d + b) = *reinterpret_cast<const uint16_t*>(a.c.k + s + b);
-            *reinterpret_cast<uint16_t*>(a.to.v + d + b) = *reinterpret_cast<const uint16_t*>(a.c.v + s + b);
-        }
+#pragma unroll
+        for (uint32_t k = 0; k < MOVE_PLACES; ++k)
+            for (uint32_t b = lane * 2u; moves[k] && b < row_bytes; b += 64u) {
+                *reinterpret_cast<uint16_t*>(a.to.k + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.k + s[k] + b);
+                *reinterpret_cast<uint16_t*>(a.to.v + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.v + s[k] + b);
+            }
     }
+}
+
+cudaError_t launch_select(const EvictArgs& a, uint32_t count, uint32_t peers, size_t smem, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.c.kv_heads * peers, count);
+    cfg.blockDim = dim3(SELECT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = peers;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = m40_pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
 }
 
 }  // namespace
@@ -323,19 +466,26 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     a.ld = c->ld;
     a.bound = c->max_len ? c->max_len : capacity;
     const size_t places = (size_t)c->count * cache->kv_heads * c->keep;
-    uint32_t* work = (uint32_t*)m40_ensure_scratch(ctx, 1, 3 * places * sizeof(uint32_t), 0);
+    uint32_t* work = (uint32_t*)m40_ensure_scratch(ctx, 1, 2 * places * sizeof(uint32_t), 0);
     if (!work) return -5;
-    a.holes = work;
+    a.plan = work;
     a.late = work + places;
-    a.origin = c->origin ? c->origin : work + 2 * places;
-    cudaError_t e = m40_launch_dependent(evict_select_kernel, dim3(cache->kv_heads, c->count), dim3(SELECT_THREADS), 0, ctx->decode_stream, a);
+    a.origin = c->origin;
+    // as many CTAs for a list as fill the device once, with 1024 entries each
+    const uint64_t lists = (uint64_t)c->count * cache->kv_heads;
+    uint32_t peers = 1u;
+    while (peers < SELECT_CLUSTER && lists * peers * 2u <= (uint64_t)ctx->sm_count && a.bound > SELECT_THREADS * peers) peers *= 2u;
+    const uint32_t per = (a.bound + peers - 1u) / peers;
+    a.cached = per <= SELECT_CACHED ? per : 0u;
+    cudaError_t e = launch_select(a, c->count, peers, (size_t)a.cached * (c->entry_pos ? 8u : 4u), ctx->decode_stream);
     M40_COUNT_LAUNCH(ctx);
-    if (e != cudaSuccess) return -3;
+    if (e != cudaSuccess) return cudaGetLastError(), -3;
     const uint32_t elem = cache->elem_dtype == M40LLM_DT_F32 ? 4u : 2u;
-    e = m40_launch_dependent(evict_move_kernel, dim3((c->keep + 7u) / 8u, cache->kv_heads, c->count), dim3(256), 0, ctx->decode_stream, a,
-                             cache->head_dim * elem, elem, m40_paged_vec16(cache) && m40_paged_vec16(to) ? 1u : 0u);
+    e = m40_launch_dependent(evict_move_kernel, dim3((c->keep + 8u * MOVE_PLACES - 1u) / (8u * MOVE_PLACES), cache->kv_heads, c->count), dim3(256), 0,
+                             ctx->decode_stream, a, cache->head_dim * elem, elem, m40_paged_vec16(cache) && m40_paged_vec16(to) ? 1u : 0u);
     M40_COUNT_LAUNCH(ctx);
-    return e == cudaSuccess && cudaGetLastError() == cudaSuccess ? 0 : -3;
+    if (e != cudaSuccess) return cudaGetLastError(), -3;
+    return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 }  // extern "C"
