@@ -96,9 +96,9 @@ struct EvictArgs {
     uint32_t cached;    // entries that a CTA's shared memory holds
 };
 
-constexpr uint32_t SELECT_THREADS = 1024, SELECT_WARPS = SELECT_THREADS / 32, EVICT_HOLE = 0x80000000u, SELECT_CLUSTER = 8;
-constexpr uint32_t SELECT_CACHED = 24576;  // entries with key and position in 192 KB
-constexpr int SELECT_BITS = 11, SELECT_BINS = 1 << SELECT_BITS, SELECT_PASSES = 3;  // 32 bits in 11, 11 and 10
+constexpr uint32_t SELECT_THREADS = 512, SELECT_WARPS = SELECT_THREADS / 32, EVICT_HOLE = 0x80000000u, SELECT_CLUSTER = 16;
+constexpr uint32_t SELECT_CACHED = 24576;  // entries with key and position or list in 192 KB
+constexpr int SELECT_BITS = 11, SELECT_BINS = 1 << SELECT_BITS, SELECT_GROUPS = SELECT_BINS / 32, SELECT_PASSES = 3;  // 32 bits in 11, 11 and 10
 
 // Larger is better. Held entries come before every weight (+inf is 0xff800000), NaN after every other.
 __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
@@ -114,7 +114,7 @@ __device__ __forceinline__ uint4 warps_before(const uint4& mine, uint4* warps, u
     __syncthreads();
     if (lane == 0) warps[warp] = mine;
     __syncthreads();
-    const uint4 x = warps[lane];  // SELECT_WARPS is 32
+    const uint4 x = lane < SELECT_WARPS ? warps[lane] : make_uint4(0, 0, 0, 0);
     const auto upto = [&](uint32_t v, uint32_t* all) {
         uint32_t sum = v;
 #pragma unroll
@@ -131,10 +131,11 @@ __device__ __forceinline__ uint4 warps_before(const uint4& mine, uint4* warps, u
 }
 
 struct SelectShared {
-    uint32_t bins[SELECT_PASSES][SELECT_BINS];  // one set per pass: a pass needs no barrier after its counts were read
+    uint32_t bins[SELECT_PASSES][SELECT_BINS];     // one set per pass: a pass needs no barrier after its counts were read
+    uint32_t groups[SELECT_PASSES][SELECT_GROUPS];  // sums of 32 bins
     uint4 warps[SELECT_WARPS];
     uint4 counts;                               // this CTA's: larger and equal keys below the new end, then behind it
-    uint32_t newest, pick[2];
+    uint32_t newest, listed, pick[2];
 };
 
 // Cluster of CTAs = (listed sequence, kv head); a CTA has a run of its entries, their keys in shared memory where they fit (else they are made again in every
@@ -143,13 +144,13 @@ struct SelectShared {
 // holes and kept entries behind the end, so that the plan is written without an order of who comes first. Against one CTA and four passes from memory: 4 x 8
 // heads of 8192 entries 68 -> @E us, 8 heads of 32768 200 -> @F. Bound by the barriers of the cluster.
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs a) {
-    extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions
+    extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions, then the keys that later passes look at
     __shared__ SelectShared sh;
     uint32_t peers;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
     const uint32_t me = tc::cluster_rank(), h = blockIdx.x / peers, i = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     for (uint32_t b = tid; b < SELECT_PASSES * SELECT_BINS; b += SELECT_THREADS) (&sh.bins[0][0])[b] = 0u;
-    if (tid == 0) sh.newest = 0u;
+    if (tid == 0) sh.newest = 0u, sh.listed = 0u;
     pdl_wait();
     pdl_trigger();
     const uint32_t slot = a.seq[i], len = a.len[i];
@@ -177,9 +178,10 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     const bool cached = per <= a.cached;
     uint32_t* s_key = s_dyn;
     uint32_t* s_pos = s_dyn + a.cached;
+    uint32_t* s_list = s_pos;
     uint32_t newest = 0;
     if (pos) {
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t j = tid; j < mine; j += SELECT_THREADS) {
             const uint32_t p = pos[lo + j];
             if (cached) s_pos[j] = p, s_key[j] = evict_key(w[lo + j], false);
@@ -199,6 +201,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
         return evict_key(w[e], p < a.first || newest - p < a.recent);
     };
     if (cached)
+#pragma unroll 8
         for (uint32_t j = tid; j < mine; j += SELECT_THREADS) {
             if (!pos) {
                 s_key[j] = fresh(lo + j);
@@ -215,45 +218,87 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
         const int shift = pass == 0 ? 32 - SELECT_BITS : (pass == 1 ? 32 - 2 * SELECT_BITS : 0), bits = pass == 2 ? 32 - 2 * SELECT_BITS : SELECT_BITS;
         const uint32_t high = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
         uint32_t* bins = sh.bins[pass];
-        // the thread's own keys: it made them. Lanes that meet in a bin add once.
-        for (uint32_t j0 = 0; j0 < mine; j0 += SELECT_THREADS) {
+        // Pass 0: the thread's own keys; then, where keys are kept, those that begin with the prefix are listed. A warp whose keys are all in one bin (equal
+        // weights) adds once.
+        const bool listed = pass > 0 && cached;
+        const uint32_t n = listed ? sh.listed : mine;
+        for (uint32_t j0 = 0; j0 < n; j0 += SELECT_THREADS) {
             const uint32_t j = j0 + tid;
-            const uint32_t k = j < mine ? key(lo + j) : 0u;
-            const bool in = j < mine && (k & high) == prefix;
+            const uint32_t k = j < n ? (listed ? s_list[j] : key(lo + j)) : 0u;
+            const bool in = j < n && (k & high) == prefix;
             const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
-            const uint32_t same = __match_any_sync(0xffffffffu, in ? bin : 0xffffffffu);
-            if (in && (same & ((1u << lane) - 1u)) == 0u) atomicAdd(&bins[bin], (uint32_t)__popc(same));
+            const uint32_t active = __ballot_sync(0xffffffffu, in);
+            if (active == 0u) continue;
+            const uint32_t leader = __ffs(active) - 1u, its = __shfl_sync(0xffffffffu, bin, leader);
+            if (__all_sync(0xffffffffu, !in || bin == its)) {
+                if (lane == leader) atomicAdd(&bins[bin], (uint32_t)__popc(active));
+            } else if (in) {
+                atomicAdd(&bins[bin], 1u);
+            }
+        }
+        __syncthreads();
+        constexpr uint32_t RUN = SELECT_BINS / SELECT_THREADS;  // the thread's bins, for the groups' sums
+        static_assert(RUN == 4u, "eight threads have a group of 32 bins");
+        {
+            const uint4 x = *reinterpret_cast<const uint4*>(bins + RUN * tid);
+            uint32_t sum = x.x + x.y + x.z + x.w;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            if ((tid & 7u) == 0) sh.groups[pass][tid / 8u] = sum;
         }
         __syncthreads();
         if (peers > 1u) tc::cluster_sync_all();
-        // thread t: the bins from the top, 2 t and 2 t + 1
-        constexpr uint32_t top = SELECT_BINS - 1;
-        uint32_t n0 = 0, n1 = 0;
-        const uint32_t at = tc::smem_u32(bins + (top - 2u * tid - 1u));
+        if (warp == 0) {
+            // the group, then the bin in it, each from the top: all of the bins from all CTAs took 3750 of a pass's 8000 cycles
+            const auto before_lane = [&](uint32_t own) {
+                uint32_t sum = own;
 #pragma unroll
-        for (uint32_t c = 0; c < SELECT_CLUSTER; ++c)
-            if (c < peers) {
-                const uint2 n = tc::ld_cluster2(tc::map_to_rank(at, c));
-                n0 += n.y, n1 += n.x;
-            }
-        uint32_t sum = n0 + n1;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= (uint32_t)o) sum += u;
+                }
+                return sum - own;
+            };
+            static_assert(SELECT_GROUPS == 64, "two groups a lane");
+            uint32_t g0 = 0, g1 = 0;  // the lane's lower and upper group
+            const uint32_t g_at = tc::smem_u32(&sh.groups[pass][SELECT_GROUPS - 2u * (lane + 1u)]);
+            uint2 from[SELECT_CLUSTER];  // all loads on their way before the first is added
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= (uint32_t)o) sum += u;
-        }
-        if (lane == 31u) sh.warps[warp].x = sum;
-        __syncthreads();
-        uint32_t above = lane < warp ? sh.warps[lane].x : 0u;
-        above = __reduce_add_sync(0xffffffffu, above) + sum - n0 - n1;  // entries in the bins above this thread's
-        if (above < want && above + n0 + n1 >= want) {
-            const bool upper = above + n0 >= want;
-            sh.pick[0] = top - 2u * tid - (upper ? 0u : 1u);
-            sh.pick[1] = want - above - (upper ? 0u : n0);
+            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) from[c] = c < peers ? tc::ld_cluster2(tc::map_to_rank(g_at, c)) : make_uint2(0u, 0u);
+#pragma unroll
+            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) g0 += from[c].x, g1 += from[c].y;
+            uint32_t above = before_lane(g0 + g1);
+            const uint32_t owner = __ffs(__ballot_sync(0xffffffffu, above < want && above + g0 + g1 >= want)) - 1u;
+            const bool lower = above + g1 < want;
+            if (lower) above += g1;
+            const uint32_t group = __shfl_sync(0xffffffffu, SELECT_GROUPS - 1u - 2u * lane - (lower ? 1u : 0u), owner);
+            above = __shfl_sync(0xffffffffu, above, owner);
+            uint32_t own = 0;
+            const uint32_t bin = group * 32u + 31u - lane, b_at = tc::smem_u32(bins + bin);
+#pragma unroll
+            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) from[c].x = c < peers ? tc::ld_cluster(tc::map_to_rank(b_at, c)) : 0u;
+#pragma unroll
+            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) own += from[c].x;
+            above += before_lane(own);
+            if (above < want && above + own >= want) sh.pick[0] = bin, sh.pick[1] = want - above;
         }
         __syncthreads();
         prefix |= sh.pick[0] << shift;
         want = sh.pick[1];
+        if (pass == 0 && cached) {  // the positions are done with
+            for (uint32_t j0 = 0; j0 < mine; j0 += SELECT_THREADS) {
+                const uint32_t j = j0 + tid, k = j < mine ? s_key[j] : 0u;
+                const bool in = j < mine && (k >> shift) == sh.pick[0];
+                const uint32_t active = __ballot_sync(0xffffffffu, in);
+                if (active == 0u) continue;
+                uint32_t first = 0;
+                if (lane == __ffs(active) - 1u) first = atomicAdd(&sh.listed, (uint32_t)__popc(active));
+                first = __shfl_sync(0xffffffffu, first, __ffs(active) - 1u);
+                if (in) s_list[first + __popc(active & ((1u << lane) - 1u))] = k;
+            }
+            __syncthreads();
+        }
     }
 
     uint4 count = make_uint4(0, 0, 0, 0);  // larger, equal below the new end; larger, equal behind it
@@ -372,6 +417,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t r
 
 cudaError_t launch_select(const EvictArgs& a, uint32_t count, uint32_t peers, size_t smem, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && peers > 8u) e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.c.kv_heads * peers, count);
@@ -471,13 +517,13 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     a.plan = work;
     a.late = work + places;
     a.origin = c->origin;
-    // as many CTAs for a list as fill the device once, with 1024 entries each
+    // as many CTAs for a list as fill the device once, with 512 entries or more each
     const uint64_t lists = (uint64_t)c->count * cache->kv_heads;
     uint32_t peers = 1u;
     while (peers < SELECT_CLUSTER && lists * peers * 2u <= (uint64_t)ctx->sm_count && a.bound > SELECT_THREADS * peers) peers *= 2u;
     const uint32_t per = (a.bound + peers - 1u) / peers;
     a.cached = per <= SELECT_CACHED ? per : 0u;
-    cudaError_t e = launch_select(a, c->count, peers, (size_t)a.cached * (c->entry_pos ? 8u : 4u), ctx->decode_stream);
+    cudaError_t e = launch_select(a, c->count, peers, (size_t)a.cached * 8u, ctx->decode_stream);
     M40_COUNT_LAUNCH(ctx);
     if (e != cudaSuccess) return cudaGetLastError(), -3;
     const uint32_t elem = cache->elem_dtype == M40LLM_DT_F32 ? 4u : 2u;
