@@ -4,43 +4,15 @@
 // (maximum, sum, unnormalised output) meet in paged_merge_kernel in a fixed order. Where accumulated weights are asked for, the
 // scores are kept in scratch and paged_weights_kernel turns them into weights once the maximum and sum of every row are known.
 //   paged_tiles_kernel  f16 entries, head sizes 64 and 128: matrix instructions on 64-entry tiles
-//   paged_rows_kernel   any head size, group size and type: f32 multiply-adds on tiles in shared memory
-#include "attention_mma.cuh"
-#include "paged.cuh"
+//   paged_lanes_kernel  (attention_paged_lanes.cu) f32 entries and other f16 head sizes, rows in 16-byte pieces: f32 multiply-adds in registers
+//   paged_rows_kernel   what is left, odd head sizes and alignments: f32 multiply-adds on tiles in shared memory
+#include "attention_paged.cuh"
 #include "stack_math.cuh"
 
 namespace {
 
 using namespace attn_mma;
 
-struct PagedAttnArgs {
-    PagedView c;
-    const float* q;
-    float* out;
-    const uint32_t* row_slot;
-    const uint32_t* row_len;
-    const uint32_t* row_begin;
-    const float* weights_in;
-    float* weights_out;
-    float* part_m;  // [rows][q_heads][splits], base 2
-    float* part_l;
-    float* part_o;  // [rows][q_heads][splits][hd]
-    float* scores;  // [rows][q_heads][ld_scores] in base 2, or null
-    float* stat;    // [rows][q_heads][2]: maximum, 1 / sum (0 for a row without entries), where scores are kept
-    uint32_t* status;
-    uint64_t* prefix;  // paged_tiles_kernel: tiles before each row of the launch, [rows + 1]
-    uint32_t rows, q_heads, group, splits, chunk, bound, ld_weights, ld_scores;
-    uint32_t row0, heads_at_once, workers;  // paged_tiles_kernel: first row of the launch, q heads of one unit of work, warps
-    float scale;  // times log2(e)
-};
-
-// The entries [begin, end) of a row; false for a row outside the cache.
-__device__ __forceinline__ bool paged_row_range(const PagedAttnArgs& a, uint32_t row, uint32_t* slot, uint32_t* begin, uint32_t* end) {
-    *slot = a.row_slot[row];
-    *end = a.row_len[row];
-    *begin = a.row_begin ? a.row_begin[row] : 0u;
-    return *slot < a.c.slots && *end <= a.bound;
-}
 // The part of them that split s covers: whole tiles of 64, counted from the one that `begin` lies in, dealt evenly to the splits, at least a.chunk
 // entries to each that has any.
 __device__ __forceinline__ void paged_chunk(const PagedAttnArgs& a, uint32_t split, uint32_t begin, uint32_t end, uint32_t* t0, uint32_t* t1) {
@@ -58,7 +30,7 @@ constexpr uint32_t ROWS_THREADS = 128;
 // (entry, slice of the dimensions), the slices meet in shared memory; softmax: warp = head, lane = entry; output: thread = dimensions.
 template <typename ET, int GT, int DV>
 __global__ void __launch_bounds__(ROWS_THREADS) paged_rows_kernel(PagedAttnArgs a, uint32_t T, uint32_t vec, uint32_t pitch) {
-    extern __shared__ __align__(16) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, hd = a.c.hd, hd4 = (hd + 3u) & ~3u;
     float* s_q = reinterpret_cast<float*>(smem);                 // [GT][hd4]
     float* s_part = s_q + GT * hd4;                              // [slices][GT][T]
@@ -270,10 +242,6 @@ __device__ __noinline__ void paged_plain_run(const PagedAttnArgs& a, uint32_t sl
     for (int j = 0; j < HD / 64; ++j) *reinterpret_cast<float2*>(o_out + d + 64 * j) = make_float2(o[2 * j], o[2 * j + 1]);
 }
 
-// 16 bytes by cp.async; zeros where `bytes` is 0 (the source is then not read)
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes));
-}
 __device__ __forceinline__ void ldmatrix_at(uint32_t (&r)[4], uint32_t smem) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
@@ -287,30 +255,19 @@ __device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t sme
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
 
-// The work of a launch is a list of tiles of 16 entries: rows in order, in a row the units of up to 8 (WIDE: 16) q heads of one kv head, in a unit
-// its tiles. Every warp takes an equal run of the list, with a ring of its own and without a barrier, so that no warp waits for another, none starts late and
-// none ends early, whatever the lengths. A warp leaves a part (maximum, sum, output) of every unit that its run touches, and paged_join_kernel puts the parts
-// together: the part of warp w in unit u of all units is number u + w, which no other has, as w or u grows from one part of the list to the next. Against one
-// CTA per (row, unit, 1024 entries) with barriers: 32 rows of up to 16384 entries 198 -> @A us, one of 130001 110 -> @B.
+// A run of the list of work per CTA, tiles of 64 entries; a warp takes 16 of them, with a ring of its own. Against one CTA per (row, unit, 1024
+// entries): 32 rows of up to 16384 entries 198 -> 173 us, one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
+// and without a barrier per tile the warps drift apart: 187 and 179 us for the 32 rows.
 //   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units.
 //   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them. A group has
 //                         at most 8 heads as a rule: hi and lo are then the two halves of the 16 rows of ONE operand, and the halves of the result are
 //                         added (WIDE: two products).
 //   softmax               online in base 2; the outputs are rescaled only when a maximum moved.
-constexpr uint32_t TILES_ROWS = 256;  // rows of a launch: their ranges stay in shared memory
-
-// The warp whose run holds tile x of `total`; warp i of n has [i total / n, (i + 1) total / n).
-__device__ __forceinline__ uint64_t quotient(uint64_t x, uint64_t y) {  // most lists are short enough for the fast division
-    return (x | y) >> 32 ? x / y : (uint64_t)((uint32_t)x / (uint32_t)y);
-}
-__device__ __forceinline__ uint32_t warp_of(uint64_t x, uint64_t total, uint32_t n) { return (uint32_t)quotient((x + 1u) * n - 1u, total); }
-__device__ __forceinline__ uint32_t warps_at_work(uint64_t total, uint32_t n) { return total < n ? (uint32_t)total : n; }
-
 template <int HD, bool WIDE>
 struct TilesCfg {
     static constexpr int STAGES = HD == 128 ? 3 : 4, CTAS = HD == 128 ? 2 : 3;
     static constexpr int STAGE = 2 * (int)TILE * HD * 2;                                                                    // K and V of a tile
-    static constexpr int SMEM = 256 + (int)TILES_WARPS * STAGES * STAGE + (int)(TILES_ROWS + 1) * 8 + (int)TILES_ROWS * 12;  // rings, the prefix, the rows' ranges
+    static constexpr int SMEM = 256 + (int)TILES_WARPS * STAGES * STAGE + (int)sizeof(PagedList);  // rings, the list
 };
 
 template <int HD, bool WIDE>
@@ -318,81 +275,19 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     using Cfg = TilesCfg<HD, WIDE>;
     constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = Cfg::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* s_prefix = reinterpret_cast<uint64_t*>(smem + 256 + TILES_WARPS * STAGES * Cfg::STAGE);
-    uint32_t* s_slot = reinterpret_cast<uint32_t*>(s_prefix + TILES_ROWS + 1);
-    uint32_t* s_begin = s_slot + TILES_ROWS;
-    uint32_t* s_end = s_begin + TILES_ROWS;
+    PagedList& list = *reinterpret_cast<PagedList*>(smem + 256 + TILES_WARPS * STAGES * Cfg::STAGE);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
-    const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = min(a.rows - a.row0, TILES_ROWS);
+    const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = min(a.rows - a.row0, LIST_ROWS);
     pdl_wait();
     pdl_trigger();
-    if (tid < 32u) {  // the rows' tiles, summed up by one warp
-        uint64_t before = 0;
-        for (uint32_t r0 = 0; r0 < rows; r0 += 32u) {
-            const uint32_t r = r0 + lane;
-            uint32_t slot = 0, begin = 0, end = 0, n = 0;
-            if (r < rows) {
-                const bool inside = paged_row_range(a, a.row0 + r, &slot, &begin, &end);
-                if (!inside && blockIdx.x == 0) atomicOr(a.status, 1u);
-                n = inside && end > begin ? (end - (begin & ~(SPAN - 1u)) + SPAN - 1u) / SPAN : 0u;
-            }
-            uint32_t sum = n;  // 32 rows of at most 2^26 tiles
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= (uint32_t)o) sum += u;
-            }
-            if (r < rows) {
-                s_slot[r] = slot, s_begin[r] = begin, s_end[r] = end;
-                s_prefix[r] = before + sum - n;
-                if (blockIdx.x == 0) a.prefix[r] = before + sum - n;
-            }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (lane == 0) {
-            s_prefix[rows] = before;
-            if (blockIdx.x == 0) a.prefix[rows] = before;
-        }
-    }
+    if (tid < 32u) paged_list_make(a, list, rows, SPAN);
     __syncthreads();
-    const uint64_t total = s_prefix[rows] * units;
-    const uint32_t worker = blockIdx.x, workers = warps_at_work(total, a.workers);
+    const uint64_t total = list.prefix[rows] * units;
+    const uint32_t worker = blockIdx.x, workers = ctas_at_work(total, a.workers);
     if (worker >= workers) return;
     const uint64_t lo = quotient(worker * total, workers);
     const uint32_t count = (uint32_t)(quotient((worker + 1u) * total, workers) - lo);  // at least 1
-
-    // a place in the list
-    struct Place {
-        uint32_t row, unit, tile, tiles, t0, t1, first;
-    };
-    auto enter = [&](Place& p) {  // p.row has tiles
-        p.t0 = s_begin[p.row], p.t1 = s_end[p.row], p.first = p.t0 & ~(SPAN - 1u);
-        p.tiles = (p.t1 - p.first + SPAN - 1u) / SPAN;
-    };
-    auto advance = [&](Place& p) {
-        if (++p.tile < p.tiles) return false;
-        p.tile = 0;
-        if (++p.unit == units) {
-            p.unit = 0;
-            do ++p.row;
-            while (p.row < rows && s_prefix[p.row + 1] == s_prefix[p.row]);
-            if (p.row < rows) enter(p);
-        }
-        return true;
-    };
-    Place at;
-    {
-        uint32_t l = 0, h = rows;  // the last row that begins at or before lo
-        while (h - l > 1u) {
-            const uint32_t mid = (l + h) / 2u;
-            if (s_prefix[mid] * units <= lo) l = mid; else h = mid;
-        }
-        at.row = l;
-        enter(at);
-        const uint64_t in_row = lo - s_prefix[l] * units;
-        at.unit = (uint32_t)quotient(in_row, at.tiles);
-        at.tile = (uint32_t)(in_row - (uint64_t)at.unit * at.tiles);
-    }
+    PagedPlace at = paged_list_at(list, lo, rows, units, SPAN);
 
     // The lane copies piece `ch` of rows my_row, my_row + ROWS_AT_ONCE, ..; the swizzle of row r is r mod 8.
     constexpr uint32_t ROWS_AT_ONCE = 32u / CHUNKS, COPIES = TILE / ROWS_AT_ONCE, toSV = TILE * HD * 2u;
@@ -403,12 +298,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     const uint64_t page_bytes = a.c.kv_heads * head_bytes;
     const ptrdiff_t toV = a.c.v - a.c.k;
     const uint32_t my_dst = ring + my_row * (HD * 2u) + ((ch ^ my_row) * 16u);  // my_row < 8; c * ROWS_AT_ONCE enters by exclusive or
-    Place fetch = at;
+    PagedPlace fetch = at;
     const uint32_t* pages = nullptr;
     const unsigned char* srcK = nullptr;
     bool bad = false;  // the warp met a page outside the pool
     auto aim = [&]() {
-        pages = a.c.table + (size_t)s_slot[fetch.row] * a.c.max_pages;
+        pages = a.c.table + (size_t)list.slot[fetch.row] * a.c.max_pages;
         srcK = a.c.k + fetch.unit / subgroups * head_bytes + ch * 16u;
     };
     auto load = [&](uint32_t f) {  // tile f of the run, where `fetch` is
@@ -440,7 +335,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                 cp_async16_or_zero(to + toSV, ok ? src + toV : a.c.v, ok ? 16u : 0u);
             }
         }
-        if (advance(fetch) && f + 1u < count) aim();
+        if (paged_list_next(list, fetch, rows, units, SPAN) && f + 1u < count) aim();
     };
     aim();
 #pragma unroll
@@ -521,7 +416,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             s[h][2] = WIDE ? s1[0][2 * h] : s1[0][0] + s1[0][2], s[h][3] = WIDE ? s1[0][2 * h + 1] : s1[0][1] + s1[0][3];
         }
         if (base < at.t0 || base + TILE > at.t1 || __any_sync(0xffffffffu, bad)) {
-            const uint32_t* own_pages = a.c.table + (size_t)s_slot[at.row] * a.c.max_pages;
+            const uint32_t* own_pages = a.c.table + (size_t)list.slot[at.row] * a.c.max_pages;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t e = e0 + (i & 1) + (i >> 1) * 8;
@@ -615,13 +510,13 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                     odd &= ~(0xfu << (4u * gh));
                     const size_t at_part = part + gh + 8u * h, at_head = (size_t)row * a.q_heads + head;
                     __syncwarp();
-                    paged_plain_run<HD>(a, s_slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
+                    paged_plain_run<HD>(a, list.slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
                                           max(at.t0, at.first + tile_begin * SPAN), min(at.t1, at.first + (at.tile + 1u) * SPAN), warp, WEIGHT_BIAS, a.part_m + at_part,
                                           a.part_l + at_part, a.part_o + at_part * HD);
                 }
             }
         }
-        entering = advance(at);
+        entering = paged_list_next(list, at, rows, units, SPAN);
     }
     cp_async_wait<0>();
     if (bad) atomicOr(a.status, 1u);
@@ -709,7 +604,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
     paged_join_parts<V, LANES>(a, head, a.splits, [=](uint32_t s) { return base + s; });
 }
 
-// Parts of paged_tiles_kernel, and the zeros of rows without entries. Grid (q head, row of the launch, share of the dimensions).
+// Parts of paged_tiles_kernel and paged_lanes_kernel, and the zeros of rows without entries. Grid (q head, row of the launch, share of the dimensions).
 template <int LANES>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
     pdl_wait();
@@ -724,11 +619,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
             for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
         return;
     }
-    const uint32_t n = warps_at_work(total, a.workers);
+    const uint32_t n = ctas_at_work(total, a.workers);
     const uint64_t lo = before * units + unit * tiles;
-    const uint32_t w0 = warp_of(lo, total, n), w1 = warp_of(lo + tiles - 1u, total, n);
-    const size_t part = ((size_t)r * units + unit + w0) * TILES_WARPS;
-    paged_join_parts<4, LANES>(a, head, (w1 - w0 + 1u) * TILES_WARPS, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
+    const uint32_t w0 = cta_of(lo, total, n), w1 = cta_of(lo + tiles - 1u, total, n);
+    const size_t part = ((size_t)r * units + unit + w0) * a.part_warps;
+    paged_join_parts<4, LANES>(a, head, (w1 - w0 + 1u) * a.part_warps, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
 }
 
 // CTA = (1024 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
@@ -819,21 +714,27 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
 // Whether a CTA per head and row leaves most of the device idle.
 bool few_heads(const M40llmCudaContext* ctx, uint32_t q_heads, uint32_t rows) { return (uint64_t)q_heads * rows <= 2ull * (uint64_t)ctx->sm_count; }
 
-// All rows in launches of up to 256, each followed by its join.
 template <int HD, bool WIDE>
-cudaError_t launch_tiles(M40llmCudaContext* ctx, PagedAttnArgs a) {
+cudaError_t launch_tiles(M40llmCudaContext* ctx, const PagedAttnArgs& a) {
     using Cfg = TilesCfg<HD, WIDE>;
-    cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
-    const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + SPAN - 1u) / SPAN) * a.rows;
-    a.workers = (uint32_t)ctx->sm_count * Cfg::CTAS;
-    if (most < a.workers) a.workers = (uint32_t)most;
-    for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += TILES_ROWS) {
-        const uint32_t rows = a.rows - a.row0 < TILES_ROWS ? a.rows - a.row0 : TILES_ROWS;
-        e = m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM,
-                                 ctx->decode_stream, a);
+    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    if (e != cudaSuccess) return e;
+    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
+}
+
+// All rows in launches of up to 256, each followed by its join. `ctas`: how many are resident, `span`: entries of a tile of the list.
+template <typename Launch>
+cudaError_t launch_list(M40llmCudaContext* ctx, PagedAttnArgs a, uint32_t ctas, uint32_t span, Launch launch) {
+    const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + span - 1u) / span) * a.rows;
+    a.workers = most < ctas ? (uint32_t)most : ctas;
+    cudaError_t e = cudaSuccess;
+    for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += LIST_ROWS) {
+        const uint32_t rows = a.rows - a.row0 < LIST_ROWS ? a.rows - a.row0 : LIST_ROWS, hd = a.c.hd;
+        e = launch(a);
         if (e == cudaSuccess)
-            e = few_heads(ctx, a.q_heads, rows) ? m40_launch_dependent(paged_join_kernel<8>, dim3(a.q_heads, rows, HD / 32), dim3(256), 0, ctx->decode_stream, a)
-                                                : m40_launch_dependent(paged_join_kernel<32>, dim3(a.q_heads, rows), dim3(256), 0, ctx->decode_stream, a);
+            e = few_heads(ctx, a.q_heads, rows)
+                    ? m40_launch_dependent(paged_join_kernel<8>, dim3(a.q_heads, rows, (hd + 31u) / 32u), dim3(256), 0, ctx->decode_stream, a)
+                    : m40_launch_dependent(paged_join_kernel<32>, dim3(a.q_heads, rows, (hd + 127u) / 128u), dim3(256), 0, ctx->decode_stream, a);
         M40_COUNT_LAUNCH(ctx);
         M40_COUNT_LAUNCH(ctx);
     }
@@ -882,10 +783,14 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     const bool f32 = cache->elem_dtype == M40LLM_DT_F32;
     const uint32_t vec = m40_paged_vec16(cache) ? 1u : 0u;
     const bool tiles = !f32 && vec && (hd == 64u || hd == 128u) && (((uintptr_t)c->q) & 7u) == 0;
+    PagedLanes lanes = {};
+    const bool by_lanes = !tiles && (((uintptr_t)c->q) & 15u) == 0 && m40_paged_lanes(ctx, cache, a.group, &lanes), list = tiles || by_lanes;
     // heads of a group in equal shares of up to 16; 8 take one product where 9 to 16 take two
     const uint32_t shares = (a.group + 15u) / 16u;
-    a.heads_at_once = (a.group + shares - 1) / shares;
-    if (!tiles) {
+    a.heads_at_once = by_lanes ? lanes.heads_at_once : (a.group + shares - 1u) / shares;
+    a.part_warps = by_lanes ? lanes.warps : TILES_WARPS;
+    const uint32_t ctas = by_lanes ? lanes.ctas : (uint32_t)ctx->sm_count * (hd == 64u ? TilesCfg<64, false>::CTAS : TilesCfg<128, false>::CTAS);
+    if (!list) {
         const uint64_t work = (uint64_t)c->rows * cache->kv_heads * a.bound, target = 2ull * (uint64_t)ctx->sm_count;
         uint64_t chunk = (work + target - 1) / target;
         chunk = chunk < 128u ? 128u : (chunk > 1024u ? 1024u : chunk);
@@ -895,13 +800,13 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         a.splits = (uint32_t)((a.bound + chunk - 1) / chunk);
     }
     const size_t heads = (size_t)c->rows * c->q_heads;
-    if (tiles || a.splits > 1 || c->weights_out) {
+    if (list || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? (a.bound + 3u) & ~3u : 0u;
-        const size_t rows_at_once = c->rows < TILES_ROWS ? c->rows : TILES_ROWS;
-        const size_t parts = tiles ? (rows_at_once * cache->kv_heads * shares + (size_t)ctx->sm_count * (hd == 64u ? 3u : 2u)) * TILES_WARPS * a.heads_at_once
-                                   : heads * a.splits;
+        const size_t rows_at_once = c->rows < LIST_ROWS ? c->rows : LIST_ROWS;
+        const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
+        const size_t parts = list ? (rows_at_once * units + ctas) * a.part_warps * a.heads_at_once : heads * a.splits;
         const size_t floats = parts * (hd + 2) + heads * 2 + 4 + heads * (size_t)a.ld_scores;
-        const size_t prefix = (TILES_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
+        const size_t prefix = (LIST_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
         unsigned char* work_area = (unsigned char*)m40_ensure_scratch(ctx, 1, prefix + 8 + floats * sizeof(float), 0);
         if (!work_area) return -5;
         a.prefix = (uint64_t*)work_area;
@@ -915,10 +820,13 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     }
     cudaError_t e;
     if (tiles) {
-        if (hd == 64u)
-            e = a.heads_at_once <= 8u ? launch_tiles<64, false>(ctx, a) : launch_tiles<64, true>(ctx, a);
-        else
-            e = a.heads_at_once <= 8u ? launch_tiles<128, false>(ctx, a) : launch_tiles<128, true>(ctx, a);
+        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) {
+            const bool wide = x.heads_at_once > 8u;
+            return hd == 64u ? (wide ? launch_tiles<64, true>(ctx, x) : launch_tiles<64, false>(ctx, x))
+                             : (wide ? launch_tiles<128, true>(ctx, x) : launch_tiles<128, false>(ctx, x));
+        });
+    } else if (by_lanes) {
+        e = launch_list(ctx, a, ctas, 8u * lanes.warps, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
     } else {
         const uint32_t elem = f32 ? 4u : 2u, hd4 = (hd + 3u) & ~3u;
         const uint32_t T = hd4 * elem > 1024u ? 16u : 32u, pitch = ((hd4 * elem + 15u) & ~15u) / elem + 16u / elem;
