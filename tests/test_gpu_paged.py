@@ -20,13 +20,13 @@ def clean(nat):
 
 
 # ------------------------------------------------------------------------------------------------------------------ append
-def run_append(nat, c, rng, slot, entry, pos, q_heads, pairs, layout, packed, entry_arrays=True):
+def run_append(nat, c, rng, slot, entry, pos, q_heads, pairs, layout, packed, entry_arrays=True, pad=3):
     rows, kvw, qw = len(slot), c.kv_heads * c.dim, q_heads * c.dim
     q, k, v = (rng.standard_normal((rows, w)).astype(np.float32) for w in (qw, kvw, kvw))
     turns = 10000.0 ** (-np.arange(pairs) / max(1, pairs)) / (2 * np.pi)
     if packed:
-        whole = T.f32(nat, np.concatenate([q, k, v, np.full((rows, 3), 9.0, np.float32)], 1))
-        ptrs, ld = (whole.ptr, whole.ptr + 4 * qw, whole.ptr + 4 * (qw + kvw)), qw + 2 * kvw + 3
+        whole = T.f32(nat, np.concatenate([q, k, v, np.full((rows, pad), 9.0, np.float32)], 1))
+        ptrs, ld = (whole.ptr, whole.ptr + 4 * qw, whole.ptr + 4 * (qw + kvw)), qw + 2 * kvw + pad
         q_out = T.f32(nat, np.zeros((rows, max(qw, 1))))
     else:
         dq = T.f32(nat, q)
@@ -47,11 +47,24 @@ def run_append(nat, c, rng, slot, entry, pos, q_heads, pairs, layout, packed, en
                                                               (5, 5, 80, 13, 2), (2, 1, 512, 256, 8)])
 @pytest.mark.parametrize("layout,packed", [(0, True), (1, True), (1, False), (0, False)])
 def test_append(nat, kind, q_heads, kv_heads, dim, pairs, page, layout, packed):
+    check_append(nat, kind, q_heads, kv_heads, dim, pairs, page, layout, packed, 3, 0 if packed else 3)
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("q_heads,kv_heads,dim,pairs,page", [(8, 2, 64, 32, 16), (16, 2, 128, 32, 16), (4, 1, 128, 20, 1), (0, 3, 8, 4, 4), (2, 2, 72, 0, 8),
+                                                              (32, 8, 128, 64, 64), (3, 1, 512, 256, 2)])
+@pytest.mark.parametrize("layout,packed", [(0, True), (1, True), (1, False), (0, False)])
+def test_append_eights(nat, kind, q_heads, kv_heads, dim, pairs, page, layout, packed):
+    """Rows on 16 bytes, heads of eights, pairs of fours."""
+    check_append(nat, kind, q_heads, kv_heads, dim, pairs, page, layout, packed, 4, 0)
+
+
+def check_append(nat, kind, q_heads, kv_heads, dim, pairs, page, layout, packed, pad, offset):
     rng = np.random.default_rng(dim + pairs + layout)
-    c = T.Cache(nat, rng, 3, 37, kv_heads, dim, page, kind, offset=0 if packed else 3)
+    c = T.Cache(nat, rng, 3, 37, kv_heads, dim, page, kind, offset=offset)
     slot, entry = np.array([2, 0, 2, 1, 0, 2]), np.array([0, 36, 17, 5, 16, c.capacity - 1])
     pos = np.array([0, 36, 123456, 5, 4000000000, 2])
-    q, k, v, turns, q_out, ep, w = run_append(nat, c, rng, slot, entry, pos, q_heads, pairs, layout, packed)
+    q, k, v, turns, q_out, ep, w = run_append(nat, c, rng, slot, entry, pos, q_heads, pairs, layout, packed, pad=pad)
     # an angle is the product of a position and a double, whole turns dropped in double: 2^-53 of the product; sine, cosine, two products and a sum
     def bound(x):
         angle = 2 * np.pi * 2.0 ** -52 * pos[:, None, None] * (turns.max() if pairs else 0.0)
