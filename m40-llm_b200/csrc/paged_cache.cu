@@ -85,7 +85,7 @@ __device__ __forceinline__ void store4(__half* p, const float4& v) {
 }
 
 // The same for heads of eights and 16-byte aligned rows. Thread = units of eight values of a head: four pairs, or eight values that do not turn. Its loads go
-// out before the row's table is made: one after the other they took 17.4 us for 2001 rows of 20 heads of 128, now @P.
+// out before the row's table is made: one after the other they took 17.4 us for 2001 rows of 20 heads of 128, now 9.7.
 constexpr uint32_t APPEND_THREADS = 128, APPEND_UNITS = 3;
 template <typename ET>
 __global__ void __launch_bounds__(APPEND_THREADS) paged_append_vec_kernel(AppendArgs a) {
@@ -183,8 +183,9 @@ struct EvictArgs {
 };
 
 constexpr uint32_t SELECT_THREADS = 512, SELECT_WARPS = SELECT_THREADS / 32, EVICT_HOLE = 0x80000000u, SELECT_CLUSTER = 16;
-constexpr uint32_t SELECT_CACHED = 24576;  // entries with key and position or list in 192 KB
+constexpr uint32_t SELECT_CACHED = 24576;  // entries with key and position in 192 KB
 constexpr int SELECT_BITS = 11, SELECT_BINS = 1 << SELECT_BITS, SELECT_GROUPS = SELECT_BINS / 32, SELECT_PASSES = 3;  // 32 bits in 11, 11 and 10
+constexpr uint32_t SELECT_LIST = 2048;     // keys that every CTA sorts out by itself
 
 // Larger is better. Held entries come before every weight (+inf is 0xff800000), NaN after every other.
 __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
@@ -217,26 +218,48 @@ __device__ __forceinline__ uint4 warps_before(const uint4& mine, uint4* warps, u
 }
 
 struct SelectShared {
-    uint32_t bins[SELECT_PASSES][SELECT_BINS];     // one set per pass: a pass needs no barrier after its counts were read
-    uint32_t groups[SELECT_PASSES][SELECT_GROUPS];  // sums of 32 bins
+    uint32_t bins[SELECT_BINS];
     uint4 warps[SELECT_WARPS];
-    uint4 counts;                               // this CTA's: larger and equal keys below the new end, then behind it
-    uint32_t newest, listed, pick[2];
+    uint32_t newest, found, pick[4];
+    // what the CTAs of the cluster tell each other, by the teller's number
+    uint32_t newest_of[SELECT_CLUSTER];
+    uint32_t groups_of[SELECT_CLUSTER][SELECT_GROUPS];  // sums of 32 bins
+    uint32_t bins_of[SELECT_CLUSTER][32];               // one group's bins
+    uint4 counts_of[SELECT_CLUSTER];                    // larger and equal keys below the new end, then behind it
+    uint32_t list[SELECT_LIST];                         // the keys of one bin, of all CTAs
 };
 
+// All threads of the cluster; what was stored into other CTAs' memory before it is there behind it.
+__device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
+    tc::cluster_sync_all();
+}
+
+// Sum over the lanes before this one.
+__device__ __forceinline__ uint32_t lanes_before(uint32_t own) {
+    uint32_t sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((threadIdx.x & 31u) >= (uint32_t)o) sum += u;
+    }
+    return sum - own;
+}
+
 // Cluster of CTAs = (listed sequence, kv head); a CTA has a run of its entries, their keys in shared memory where they fit (else they are made again in every
-// pass). The key of the last kept entry is found by its bits from the highest down: a histogram per CTA, summed up through distributed shared memory, in every
-// CTA alike. Then the entries are counted once, larger and equal ones below and behind the new end, which gives every warp the numbers of its ties,
-// holes and kept entries behind the end, so that the plan is written without an order of who comes first. Against one CTA and four passes from memory: 4 x 8
-// heads of 8192 entries 68 -> @E us, 8 heads of 32768 200 -> @F. Bound by the barriers of the cluster.
+// pass). The key of the last kept entry is found by its bits from the highest down: a histogram of 11 bits per CTA, in groups of 32 bins; the groups' sums go to all
+// CTAs, then the bins of the one group that matters, then, where these are at most 2048, the keys of the one bin that matters, which every CTA sorts
+// out by itself (else two more histograms follow). Then the entries are counted once, larger and equal ones below and behind the new end, which gives every
+// warp the numbers of its ties, holes and kept entries behind the end, so that the plan is written without an order of who comes first. What CTAs tell each other
+// is stored into the others' memory before a barrier: loads from there took 400 cycles each. Against one CTA and four passes from memory: 4 x 8 heads
+// of 8192 entries with the copy 76 -> @E us, 8 heads of 32768 217 -> @F. Bound by the barriers of the cluster and a chain of short steps.
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs a) {
-    extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions, then the keys that later passes look at
+    extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions
     __shared__ SelectShared sh;
     uint32_t peers;
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
     const uint32_t me = tc::cluster_rank(), h = blockIdx.x / peers, i = blockIdx.y, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    for (uint32_t b = tid; b < SELECT_PASSES * SELECT_BINS; b += SELECT_THREADS) (&sh.bins[0][0])[b] = 0u;
-    if (tid == 0) sh.newest = 0u, sh.listed = 0u;
+    if (tid == 0) sh.newest = 0u, sh.found = 0u;
     pdl_wait();
     pdl_trigger();
     const uint32_t slot = a.seq[i], len = a.len[i];
@@ -264,7 +287,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     const bool cached = per <= a.cached;
     uint32_t* s_key = s_dyn;
     uint32_t* s_pos = s_dyn + a.cached;
-    uint32_t* s_list = s_pos;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // every CTA of the cluster is there before anything is stored into it
     uint32_t newest = 0;
     if (pos) {
 #pragma unroll 8
@@ -276,11 +299,13 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
         newest = __reduce_max_sync(0xffffffffu, newest);
         if (lane == 0) atomicMax(&sh.newest, newest);
         __syncthreads();
-        tc::cluster_sync_all();
-        newest = lane < peers ? tc::ld_cluster(tc::map_to_rank(tc::smem_u32(&sh.newest), lane)) : 0u;
-        newest = __reduce_max_sync(0xffffffffu, newest);
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < peers) tc::st_cluster(tc::map_to_rank(tc::smem_u32(&sh.newest_of[me]), tid), sh.newest);
+        cluster_meet();
+        newest = __reduce_max_sync(0xffffffffu, lane < peers ? sh.newest_of[lane] : 0u);
     } else {
         newest = len - 1u;
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     const auto fresh = [&](uint32_t e) {
         const uint32_t p = pos ? pos[e] : e;
@@ -299,91 +324,105 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     const auto key = [&](uint32_t e) { return cached ? s_key[e - lo] : fresh(e); };
 
     uint32_t prefix = 0, want = a.keep;  // the want-th largest among the keys that begin with prefix
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < SELECT_PASSES; ++pass) {
         const int shift = pass == 0 ? 32 - SELECT_BITS : (pass == 1 ? 32 - 2 * SELECT_BITS : 0), bits = pass == 2 ? 32 - 2 * SELECT_BITS : SELECT_BITS;
         const uint32_t high = pass == 0 ? 0u : 0xffffffffu << (shift + bits);
-        uint32_t* bins = sh.bins[pass];
-        // Pass 0: the thread's own keys; then, where keys are kept, those that begin with the prefix are listed. A warp whose keys are all in one bin (equal
-        // weights) adds once.
-        const bool listed = pass > 0 && cached;
-        const uint32_t n = listed ? sh.listed : mine;
-        for (uint32_t j0 = 0; j0 < n; j0 += SELECT_THREADS) {
-            const uint32_t j = j0 + tid;
-            const uint32_t k = j < n ? (listed ? s_list[j] : key(lo + j)) : 0u;
-            const bool in = j < n && (k & high) == prefix;
-            const uint32_t bin = (k >> shift) & ((1u << bits) - 1u);
+        for (uint32_t b = tid; b < SELECT_BINS; b += SELECT_THREADS) sh.bins[b] = 0u;
+        __syncthreads();
+        // A warp whose keys are all in one bin (equal weights) adds once.
+        for (uint32_t j0 = 0; j0 < mine; j0 += SELECT_THREADS) {
+            const uint32_t j = j0 + tid, k = j < mine ? key(lo + j) : 0u, bin = (k >> shift) & ((1u << bits) - 1u);
+            const bool in = j < mine && (k & high) == prefix;
             const uint32_t active = __ballot_sync(0xffffffffu, in);
             if (active == 0u) continue;
             const uint32_t leader = __ffs(active) - 1u, its = __shfl_sync(0xffffffffu, bin, leader);
             if (__all_sync(0xffffffffu, !in || bin == its)) {
-                if (lane == leader) atomicAdd(&bins[bin], (uint32_t)__popc(active));
+                if (lane == leader) atomicAdd(&sh.bins[bin], (uint32_t)__popc(active));
             } else if (in) {
-                atomicAdd(&bins[bin], 1u);
+                atomicAdd(&sh.bins[bin], 1u);
             }
         }
         __syncthreads();
-        constexpr uint32_t RUN = SELECT_BINS / SELECT_THREADS;  // the thread's bins, for the groups' sums
-        static_assert(RUN == 4u, "eight threads have a group of 32 bins");
+        static_assert(SELECT_BINS == 4 * SELECT_THREADS && SELECT_GROUPS == 64, "eight threads have a group, four bins each");
         {
-            const uint4 x = *reinterpret_cast<const uint4*>(bins + RUN * tid);
+            const uint4 x = *reinterpret_cast<const uint4*>(sh.bins + 4u * tid);
             uint32_t sum = x.x + x.y + x.z + x.w;
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            if ((tid & 7u) == 0) sh.groups[pass][tid / 8u] = sum;
+            const uint32_t at = tc::smem_u32(&sh.groups_of[me][tid / 8u]);
+            for (uint32_t c = tid & 7u; c < peers; c += 8u) tc::st_cluster(tc::map_to_rank(at, c), sum);
         }
-        __syncthreads();
-        if (peers > 1u) tc::cluster_sync_all();
-        if (warp == 0) {
-            // the group, then the bin in it, each from the top: all of the bins from all CTAs took 3750 of a pass's 8000 cycles
-            const auto before_lane = [&](uint32_t own) {
-                uint32_t sum = own;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= (uint32_t)o) sum += u;
-                }
-                return sum - own;
-            };
-            static_assert(SELECT_GROUPS == 64, "two groups a lane");
+        cluster_meet();
+        if (warp == 0) {  // the group, from the top, two a lane
             uint32_t g0 = 0, g1 = 0;  // the lane's lower and upper group
-            const uint32_t g_at = tc::smem_u32(&sh.groups[pass][SELECT_GROUPS - 2u * (lane + 1u)]);
-            uint2 from[SELECT_CLUSTER];  // all loads on their way before the first is added
-#pragma unroll
-            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) from[c] = c < peers ? tc::ld_cluster2(tc::map_to_rank(g_at, c)) : make_uint2(0u, 0u);
-#pragma unroll
-            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) g0 += from[c].x, g1 += from[c].y;
-            uint32_t above = before_lane(g0 + g1);
-            const uint32_t owner = __ffs(__ballot_sync(0xffffffffu, above < want && above + g0 + g1 >= want)) - 1u;
-            const bool lower = above + g1 < want;
-            if (lower) above += g1;
-            const uint32_t group = __shfl_sync(0xffffffffu, SELECT_GROUPS - 1u - 2u * lane - (lower ? 1u : 0u), owner);
-            above = __shfl_sync(0xffffffffu, above, owner);
-            uint32_t own = 0;
-            const uint32_t bin = group * 32u + 31u - lane, b_at = tc::smem_u32(bins + bin);
-#pragma unroll
-            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) from[c].x = c < peers ? tc::ld_cluster(tc::map_to_rank(b_at, c)) : 0u;
-#pragma unroll
-            for (uint32_t c = 0; c < SELECT_CLUSTER; ++c) own += from[c].x;
-            above += before_lane(own);
-            if (above < want && above + own >= want) sh.pick[0] = bin, sh.pick[1] = want - above;
+            for (uint32_t c = 0; c < peers; ++c) {
+                const uint2 x = *reinterpret_cast<const uint2*>(&sh.groups_of[c][SELECT_GROUPS - 2u * (lane + 1u)]);
+                g0 += x.x, g1 += x.y;
+            }
+            uint32_t above = lanes_before(g0 + g1);
+            if (above < want && above + g0 + g1 >= want) {
+                const bool lower = above + g1 < want;
+                sh.pick[0] = SELECT_GROUPS - 1u - 2u * lane - (lower ? 1u : 0u);
+                sh.pick[1] = above + (lower ? g1 : 0u);
+            }
         }
         __syncthreads();
-        prefix |= sh.pick[0] << shift;
-        want = sh.pick[1];
-        if (pass == 0 && cached) {  // the positions are done with
+        const uint32_t group = sh.pick[0];
+        if (tid / 32u < peers) tc::st_cluster(tc::map_to_rank(tc::smem_u32(&sh.bins_of[me][lane]), tid / 32u), sh.bins[group * 32u + lane]);
+        cluster_meet();
+        if (warp == 0) {  // the bin in it, from the top
+            uint32_t own = 0;
+            for (uint32_t c = 0; c < peers; ++c) own += sh.bins_of[c][31u - lane];
+            const uint32_t above = sh.pick[1] + lanes_before(own);
+            if (above < want && above + own >= want) sh.pick[2] = 31u - lane, sh.pick[3] = want - above;
+        }
+        __syncthreads();
+        const uint32_t in_group = sh.pick[2];
+        prefix |= (group * 32u + in_group) << shift;
+        want = sh.pick[3];
+        const uint32_t members = lane < peers ? sh.bins_of[lane][in_group] : 0u, all_members = __reduce_add_sync(0xffffffffu, members);
+        if (pass == 0 && all_members <= SELECT_LIST) {
+            const uint32_t at = __reduce_add_sync(0xffffffffu, lane < me ? members : 0u);  // where this CTA's keys go in every CTA's list
             for (uint32_t j0 = 0; j0 < mine; j0 += SELECT_THREADS) {
-                const uint32_t j = j0 + tid, k = j < mine ? s_key[j] : 0u;
-                const bool in = j < mine && (k >> shift) == sh.pick[0];
-                const uint32_t active = __ballot_sync(0xffffffffu, in);
-                if (active == 0u) continue;
-                uint32_t first = 0;
-                if (lane == __ffs(active) - 1u) first = atomicAdd(&sh.listed, (uint32_t)__popc(active));
-                first = __shfl_sync(0xffffffffu, first, __ffs(active) - 1u);
-                if (in) s_list[first + __popc(active & ((1u << lane) - 1u))] = k;
+                const uint32_t j = j0 + tid, k = j < mine ? key(lo + j) : 0u;
+                if (j < mine && (k >> shift) == (prefix >> shift)) {
+                    const uint32_t to = tc::smem_u32(sh.list + at + atomicAdd(&sh.found, 1u));
+                    for (uint32_t c = 0; c < peers; ++c) tc::st_cluster(tc::map_to_rank(to, c), k);
+                }
             }
-            __syncthreads();
+            cluster_meet();
+            // its lower 21 bits, seven at a time
+            static_assert(32 - SELECT_BITS == 21, "three times seven bits");
+#pragma unroll 1
+            for (int low = 14; low >= 0; low -= 7) {
+                if (tid < 128u) sh.bins[tid] = 0u;
+                __syncthreads();
+                for (uint32_t j = tid; j < all_members; j += SELECT_THREADS)
+                    if ((sh.list[j] >> (low + 7)) == (prefix >> (low + 7))) atomicAdd(&sh.bins[(sh.list[j] >> low) & 127u], 1u);
+                __syncthreads();
+                if (warp == 0) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(sh.bins + 124u - 4u * lane);
+                    const uint32_t own = x.x + x.y + x.z + x.w;
+                    uint32_t above = lanes_before(own);
+                    if (above < want && above + own >= want) {
+                        uint32_t bin = 127u - 4u * lane;
+                        if (above + x.w < want) {
+                            above += x.w, --bin;
+                            if (above + x.z < want) {
+                                above += x.z, --bin;
+                                if (above + x.y < want) above += x.y, --bin;
+                            }
+                        }
+                        sh.pick[2] = bin, sh.pick[3] = want - above;
+                    }
+                }
+                __syncthreads();
+                prefix |= sh.pick[2] << low;
+                want = sh.pick[3];
+            }
+            break;
         }
     }
 
@@ -396,18 +435,15 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     }
     uint4 total;
     uint4 before = warps_before(count, sh.warps, &total);
-    if (tid == 0) sh.counts = total;
-    __syncthreads();
-    if (peers > 1u) {
-        tc::cluster_sync_all();
-        uint4 other = make_uint4(0, 0, 0, 0);
-        if (lane < me) {
-            const uint32_t from = tc::map_to_rank(tc::smem_u32(&sh.counts), lane);
-            other = make_uint4(tc::ld_cluster(from), tc::ld_cluster(from + 4u), tc::ld_cluster(from + 8u), tc::ld_cluster(from + 12u));
-        }
+    if (tid < peers) {
+        const uint32_t to = tc::map_to_rank(tc::smem_u32(&sh.counts_of[me]), tid);
+        tc::st_cluster(to, total.x), tc::st_cluster(to + 4u, total.y), tc::st_cluster(to + 8u, total.z), tc::st_cluster(to + 12u, total.w);
+    }
+    cluster_meet();  // the last word between the CTAs: any may leave after it
+    {
+        const uint4 other = lane < me ? sh.counts_of[lane] : make_uint4(0, 0, 0, 0);
         before.x += __reduce_add_sync(0xffffffffu, other.x), before.y += __reduce_add_sync(0xffffffffu, other.y);
         before.z += __reduce_add_sync(0xffffffffu, other.z), before.w += __reduce_add_sync(0xffffffffu, other.w);
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read what it needs of the others
     }
     // Entries below the end come before those behind it, so the ties, kept entries and holes before the warp follow from the four counts. As the first
     // `want` ties stay: below the end, kept = larger + min(ties, want).
@@ -433,7 +469,6 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
         holes += __popc(hole_mask);
         late += __popc(late_mask);
     }
-    if (peers > 1u) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // no CTA leaves while its counts are read
 }
 
 // Warp = MOVE_PLACES kept places of one kv head, their loads on their way together. In place a source lies behind the new end and a target before it, so
