@@ -252,7 +252,7 @@ __device__ __forceinline__ uint32_t lanes_before(uint32_t own) {
 // out by itself (else two more histograms follow). Then the entries are counted once, larger and equal ones below and behind the new end, which gives every
 // warp the numbers of its ties, holes and kept entries behind the end, so that the plan is written without an order of who comes first. What CTAs tell each other
 // is stored into the others' memory before a barrier: loads from there took 400 cycles each. Against one CTA and four passes from memory: 4 x 8 heads
-// of 8192 entries with the copy 76 -> @E us, 8 heads of 32768 217 -> @F. Bound by the barriers of the cluster and a chain of short steps.
+// of 8192 entries with the copy 76 -> 24 us, 8 heads of 32768 217 -> 28.5. Bound by the barriers of the cluster and a chain of short steps.
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs a) {
     extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions
     __shared__ SelectShared sh;
@@ -650,6 +650,12 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     const uint32_t per = (a.bound + peers - 1u) / peers;
     a.cached = per <= SELECT_CACHED ? per : 0u;
     cudaError_t e = launch_select(a, c->count, peers, (size_t)a.cached * 8u, ctx->decode_stream);
+    if (e != cudaSuccess && peers > 8u) {  // a device that has no room for clusters of more than 8
+        cudaGetLastError();
+        peers = 8u;
+        a.cached = (a.bound + peers - 1u) / peers <= SELECT_CACHED ? (a.bound + peers - 1u) / peers : 0u;
+        e = launch_select(a, c->count, peers, (size_t)a.cached * 8u, ctx->decode_stream);
+    }
     M40_COUNT_LAUNCH(ctx);
     if (e != cudaSuccess) return cudaGetLastError(), -3;
     const uint32_t elem = cache->elem_dtype == M40LLM_DT_F32 ? 4u : 2u;

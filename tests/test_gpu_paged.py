@@ -311,6 +311,34 @@ def test_attention_captured(nat):
         L.m40llm_cuda_graph_destroy(graph)
 
 
+@pytest.mark.parametrize("kind,dim", [("f16", 128), ("f16", 64), ("f32", 64), ("f16", 96)])
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_attention_queries_anywhere(nat, kind, dim, shift):
+    """Queries that lie on 4, 8 and 12 bytes behind a 16-byte boundary."""
+    rng = np.random.default_rng(shift)
+    c = T.Cache(nat, rng, 2, 200, 2, dim, 16, kind)
+    q = rng.standard_normal((2, 6, dim)).astype(np.float32)
+    desc, call, out, _ = T.attention_call(nat, c, q, [1, 0], [200, 33])
+    call.q = T.f32(nat, np.concatenate([np.zeros(shift), q.ravel()])).ptr + 4 * shift
+    assert nat.lib.m40llm_attention_paged_async(nat.ctx, C.byref(desc), C.byref(call)) == 0
+    nat.sync(1)
+    T.check_attention(c, q, [1, 0], [200, 33], out.download(np.float32, q.shape))
+
+
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("f32", 32)])
+def test_attention_many_rows(nat, kind, dim):
+    """More rows than a launch takes, several of a slot, with their weights."""
+    rng = np.random.default_rng(21)
+    c = T.Cache(nat, rng, 40, 150, 1, dim, 16, kind)
+    rows = 600
+    q = rng.standard_normal((rows, 2, dim)).astype(np.float32)
+    slot, length = rng.integers(0, 40, rows), rng.integers(0, 151, rows)
+    w = rng.random((40, 1, c.capacity)).astype(np.float32)
+    got, gw = T.attend(nat, c, q, slot, length, weights=w, ld=c.capacity, in_place=True)
+    T.check_attention(c, q, slot, length, got, weights=w, got_w=gw, before=w)
+    assert T.status(nat) == 0
+
+
 # ---------------------------------------------------------------------------------------------------------------- eviction
 def run_evict(nat, c, seq, length, keep, first, recent, weights, pos, to=None, in_place=True, max_len=0, origin=True):
     ld = weights.shape[2]
@@ -408,7 +436,7 @@ def test_evict_order(nat, name, positions):
     check_evict(c, [0], [n], keep, 7, 13, w, pos, got, None, False, (c.k, c.v))
 
 
-@pytest.mark.parametrize("n,keep,heads", [(30000, 4097, 3), (70000, 69999, 1), (70001, 33, 2), (1025, 1024, 1)])
+@pytest.mark.parametrize("n,keep,heads", [(30000, 4097, 3), (70000, 69999, 1), (70001, 33, 2), (1025, 1024, 1), (400001, 5000, 1)])
 def test_evict_long(nat, n, keep, heads):
     rng = np.random.default_rng(n)
     c = T.Cache(nat, rng, 2, n, heads, 8, 128, spare=1)
@@ -452,6 +480,37 @@ def test_evict_outside(nat):
             dst = (c.table[0, e // 16], h, e % 16)
             src = dst if o >= 144 else (c.table[0, o // 16], h, o % 16)
             assert np.array_equal(gk[dst], c.k[src])
+
+
+def test_evict_captured(nat):
+    """A captured eviction is replayed on other weights and lengths."""
+    rng = np.random.default_rng(31)
+    c = T.Cache(nat, rng, 3, 2500, 2, 16, 16)
+    keep, L = 700, nat.lib
+    w = heavy_tailed(rng, (3, 2, c.capacity))
+    d_w, d_len, d_seq = T.f32(nat, w), T.u32(nat, [9, 9, 9]), T.u32(nat, [2, 0, 1])
+    w_out, origin, new = T.f32(nat, w), T.u32(nat, np.zeros((3, 2, keep))), T.u32(nat, np.zeros(3))
+    to = T.Cache(nat, rng, 3, keep, 2, 16, 64)
+    desc, dto = c.desc(), to.desc()
+    call = N.PagedEvict(C.addressof(dto), d_seq.ptr, d_len.ptr, d_w.ptr, w_out.ptr, None, None, origin.ptr, new.ptr, 3, keep, 3, 50, c.capacity, 0)
+    run = lambda: L.m40llm_paged_evict_async(nat.ctx, C.byref(desc), C.byref(call))  # noqa: E731
+    assert run() == 0
+    nat.sync(1)
+    graph = C.c_void_p()
+    assert L.m40llm_cuda_graph_begin_capture(nat.ctx, 1) == 0
+    assert run() == 0
+    assert L.m40llm_cuda_graph_end_capture(nat.ctx, 1, C.byref(graph)) == 0
+    for lens in ([2500, 700, 1], [0, 701, 1999]):
+        w = heavy_tailed(rng, w.shape)
+        d_w.upload(w)
+        d_len.upload(np.array(lens, np.uint32))
+        w_out.upload(np.full(w.shape, -5.0, np.float32))
+        before = to.download()
+        assert L.m40llm_cuda_graph_launch(nat.ctx, graph, 1) == 0
+        nat.sync(1)
+        got = origin.download(np.uint32, (3, 2, keep)), new.download(np.uint32, 3), w_out.download(np.float32, w.shape), None
+        check_evict(c, [2, 0, 1], lens, keep, 3, 50, w, None, got, to, False, before)
+    L.m40llm_cuda_graph_destroy(graph)
 
 
 # ------------------------------------------------------------------------------------------------------------- all together
