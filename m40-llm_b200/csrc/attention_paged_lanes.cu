@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
             const bool ok = pg < a.c.pages;
             bad |= !ok;
             const unsigned char* src = srcK + (ok ? pg * page_bytes : 0) + (size_t)(base & in_page) * rb;
+#pragma unroll 4
             for (uint32_t p = lane; p < LANES_TILE * pieces; p += 32u) {
                 cp_async16_or_zero(dst + p * 16u, src + p * 16u, ok ? 16u : 0u);
                 cp_async16_or_zero(dst + tile_bytes + p * 16u, src + toV + p * 16u, ok ? 16u : 0u);
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
             for (int h = 0; h < HPL; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
         }
         cp_async_wait<LANES_STAGES - 2>();
-        __syncthreads();
+        __syncwarp();
         if (f + LANES_STAGES - 1u < count) load(f + LANES_STAGES - 1u);
         cp_async_commit();
         const uint32_t base = at.first + at.tile * span + warp * LANES_TILE;
