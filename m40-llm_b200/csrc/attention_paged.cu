@@ -527,21 +527,35 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
 // head's dimensions where there are few heads, for more loads at a time.
 template <int V, int LANES, typename Part>
 __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t parts, Part part) {
-    constexpr uint32_t MOST = 1792, GROUPS = 256 / LANES;
+    constexpr uint32_t MOST = 1792, GROUPS = 256 / LANES, AT_ONCE = 4;
     __shared__ float sw[MOST], red[16];
-    __shared__ float s_acc[GROUPS][LANES * V];
+    __shared__ float s_acc[8][LANES * V];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
+    const uint32_t vl = tid % LANES, group = tid / LANES, d = (blockIdx.z * LANES + vl) * V;
+    float x[AT_ONCE][V];
+    const auto fetch = [&](uint32_t s0) {
+#pragma unroll
+        for (uint32_t k = 0; k < AT_ONCE; ++k) {
+            const uint32_t s = s0 + k * GROUPS;
+            if (s >= parts || d >= hd) continue;
+            const float* src = a.part_o + part(s) * hd + d;
+            if constexpr (V == 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src);
+                x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+            } else {
+                x[k][0] = src[0];
+            }
+        }
+    };
+    fetch(group);  // on their way while the weights are made
     float m[MOST / 256], l[MOST / 256], M = -INFINITY, L = 0.0f;
 #pragma unroll
     for (uint32_t j = 0; j < MOST / 256u; ++j) {
         const uint32_t s = tid + 256u * j;
         m[j] = -INFINITY, l[j] = 0.0f;
         if (256u * j >= parts) continue;
-        if (s < parts) {
-            l[j] = a.part_l[part(s)];
-            if (l[j] != 0.0f) m[j] = a.part_m[part(s)];
-        }
-        M = fmaxf(M, m[j]);
+        if (s < parts) l[j] = a.part_l[part(s)], m[j] = a.part_m[part(s)];
+        M = fmaxf(M, m[j]);  // an empty part's is -inf
     }
     M = warp_max(M);
     if (lane == 0) red[warp] = M;
@@ -563,34 +577,34 @@ __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t 
 #pragma unroll
     for (int i = 0; i < 8; ++i) L += red[8 + i];
     if (a.stat && tid == 0 && blockIdx.z == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
-    const uint32_t vl = tid % LANES, group = tid / LANES, d = (blockIdx.z * LANES + vl) * V;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    if (d < hd) {
-#pragma unroll 4
-        for (uint32_t s = group; s < parts; s += GROUPS) {
-            const float w = sw[s];
-            const float* src = a.part_o + part(s) * hd + d;
-            float x[V];
-            if constexpr (V == 4) {
-                const float4 y = *reinterpret_cast<const float4*>(src);
-                x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-            } else {
-                x[0] = src[0];
-            }
-            if (w != 0.0f)  // an empty part's outputs may be anything
+    for (uint32_t s0 = group; s0 < parts; s0 += AT_ONCE * GROUPS) {
+        if (s0 != group) fetch(s0);
+        if (d < hd)
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[i], acc[i]);
-        }
+            for (uint32_t k = 0; k < AT_ONCE; ++k) {
+                const uint32_t s = s0 + k * GROUPS;
+                const float w = s < parts ? sw[s] : 0.0f;
+                if (w != 0.0f)  // an empty part's outputs may be anything
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[i] = fmaf(w, x[k][i], acc[i]);
+            }
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_acc[group][i * LANES + vl] = acc[i];
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int o = LANES; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    if (lane < LANES)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_acc[warp][i * LANES + lane] = acc[i];
     __syncthreads();
     if (tid < LANES * V) {  // value tid: i = tid / LANES of lane tid % LANES
         const uint32_t at = (blockIdx.z * LANES + tid % LANES) * V + tid / LANES;
         float o = 0.0f;
-        for (int g = 0; g < (int)GROUPS; ++g) o += s_acc[g][tid];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) o += s_acc[w][tid];
         if (at < hd) a.out[head * hd + at] = L == 0.0f ? 0.0f : o / L;
     }
 }

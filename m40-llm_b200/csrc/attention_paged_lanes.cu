@@ -155,14 +155,12 @@ __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
                 const ET* kr = tK + (half * 4u + (i ^ turn)) * hd;
                 uint64_t s[GT];
 #pragma unroll
-                for (int j = 0; j < GT; ++j) s[j] = 0u;
-#pragma unroll
                 for (uint32_t c = 0; c < DQ; ++c) {
                     const uint32_t d = (slice + 16u * c) * 4u;
                     uint64_t k[2] = {0u, 0u};
                     if (d < hd) load4(kr + d, k);
 #pragma unroll
-                    for (int j = 0; j < GT; ++j) s[j] = fma2(q[j][2 * c + 1], k[1], fma2(q[j][2 * c], k[0], s[j]));
+                    for (int j = 0; j < GT; ++j) s[j] = fma2(q[j][2 * c + 1], k[1], c == 0 ? mul2(q[j][0], k[0]) : fma2(q[j][2 * c], k[0], s[j]));
                 }
 #pragma unroll
                 for (int j = 0; j < GT; ++j) {
