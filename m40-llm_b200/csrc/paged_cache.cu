@@ -393,30 +393,36 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
                 }
             }
             cluster_meet();
-            // its lower 21 bits, seven at a time
-            static_assert(32 - SELECT_BITS == 21, "three times seven bits");
+            // its lower 21 bits, 11 and 10 at a time
+            static_assert(SELECT_BITS == 11, "21 bits are left");
 #pragma unroll 1
-            for (int low = 14; low >= 0; low -= 7) {
-                if (tid < 128u) sh.bins[tid] = 0u;
+            for (int low = 10; low >= 0; low -= 10) {
+                const int width = low ? 11 : 10;
+                *reinterpret_cast<uint4*>(sh.bins + 4u * tid) = make_uint4(0, 0, 0, 0);
                 __syncthreads();
-                for (uint32_t j = tid; j < all_members; j += SELECT_THREADS)
-                    if ((sh.list[j] >> (low + 7)) == (prefix >> (low + 7))) atomicAdd(&sh.bins[(sh.list[j] >> low) & 127u], 1u);
+                for (uint32_t j = tid; j < all_members; j += SELECT_THREADS) {
+                    const uint32_t k = sh.list[j];
+                    if ((k >> (low + width)) == (prefix >> (low + width))) atomicAdd(&sh.bins[(k >> low) & ((1u << width) - 1u)], 1u);
+                }
                 __syncthreads();
-                if (warp == 0) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(sh.bins + 124u - 4u * lane);
-                    const uint32_t own = x.x + x.y + x.z + x.w;
-                    uint32_t above = lanes_before(own);
-                    if (above < want && above + own >= want) {
-                        uint32_t bin = 127u - 4u * lane;
-                        if (above + x.w < want) {
-                            above += x.w, --bin;
-                            if (above + x.z < want) {
-                                above += x.z, --bin;
-                                if (above + x.y < want) above += x.y, --bin;
-                            }
+                // thread t: four bins, from the top
+                const uint32_t lowest = SELECT_BINS - 4u * (tid + 1u);
+                const uint4 x = *reinterpret_cast<const uint4*>(sh.bins + lowest);
+                const uint32_t own = x.x + x.y + x.z + x.w;
+                uint32_t above = lanes_before(own);
+                if (lane == 31u) sh.warps[warp].x = above + own;
+                __syncthreads();
+                above += __reduce_add_sync(0xffffffffu, lane < warp ? sh.warps[lane].x : 0u);
+                if (above < want && above + own >= want) {
+                    uint32_t bin = lowest + 3u;
+                    if (above + x.w < want) {
+                        above += x.w, --bin;
+                        if (above + x.z < want) {
+                            above += x.z, --bin;
+                            if (above + x.y < want) above += x.y, --bin;
                         }
-                        sh.pick[2] = bin, sh.pick[3] = want - above;
                     }
+                    sh.pick[2] = bin, sh.pick[3] = want - above;
                 }
                 __syncthreads();
                 prefix |= sh.pick[2] << low;
