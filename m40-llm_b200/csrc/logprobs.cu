@@ -161,9 +161,11 @@ struct LpRow {
     __device__ __forceinline__ LpRow(const LogprobArgs& args, size_t r, uint32_t from, uint32_t n, uint32_t tok, float tok_value)
         : a(args), row(r), tid(threadIdx.x), first(from), count(n), token(tok), mine(tok_value) {
         x = a.logits + row * a.ld + first;
-        wanted = a.rank && token < a.n, ranked = wanted && mine > -INFINITY && mine < INFINITY;
-        reach = ranked ? mine : INFINITY, beyond = ranked ? lp_value(lp_key(mine) + 1u) : INFINITY;
+        wanted = a.rank && token < a.n, ranked = wanted && mine < INFINITY;
         split = token < first ? 0u : token - first;  // the token's place among these values
+        // behind a token of -inf come the values above it; before it all, NaN among them, which no comparison counts
+        reach = mine > -INFINITY ? mine : NAN, beyond = ranked ? lp_value(lp_key(mine) + 1u) : INFINITY;
+        if (ranked && mine == -INFINITY && tid == 0) above = min(split, count);
         // values [0, head) and [head + 4 * fours, count) one by one, the others by fours
         head = min((4u - (uint32_t)(((uintptr_t)x >> 2) & 3u)) & 3u, count), fours = (count - head) / 4u, tail = head + 4u * fours;
         x4 = reinterpret_cast<const float4*>(x + head);

@@ -477,9 +477,9 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     }
 }
 
-// Warp = MOVE_PLACES kept places of one kv head, their loads on their way together. In place a source lies behind the new end and a target before it, so
+// Warp = MOVE_PLACES kept places of one kv head, looked up together, a lane each; four rows on their way at a time. In place a source lies behind the new end and a target before it, so
 // that no copy reads what another writes. Bound by HBM and the chain plan, late list, page tables, rows.
-constexpr uint32_t MOVE_PLACES = 4;
+constexpr uint32_t MOVE_PLACES = 8, MOVE_AT_ONCE = 4;
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t row_bytes, uint32_t elem, uint32_t vec) {
     pdl_wait();
     pdl_trigger();
@@ -507,38 +507,43 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t r
             if (a.entry_pos_out && (src != place || a.entry_pos_out != a.entry_pos)) a.entry_pos_out[base + place] = a.entry_pos ? a.entry_pos[base + src] : src;
         }
     }
-    size_t s[MOVE_PLACES], d[MOVE_PLACES];
-    bool moves[MOVE_PLACES];
+    // every lane with a place has its rows' offsets; MOVE_AT_ONCE of them move together
+    const bool moving = from != PAGED_NONE;
+    const size_t own_s = moving ? paged_row(a.c, from, h, src) * elem : 0, own_d = moving ? paged_row(a.to, into, h, place) * elem : 0;
+    const uint32_t mask = __ballot_sync(0xffffffffu, moving);
+    for (uint32_t k0 = 0; k0 < MOVE_PLACES; k0 += MOVE_AT_ONCE) {
+        if (((mask >> k0) & ((1u << MOVE_AT_ONCE) - 1u)) == 0u) continue;
+        size_t s[MOVE_AT_ONCE], d[MOVE_AT_ONCE];
+        bool moves[MOVE_AT_ONCE];
 #pragma unroll
-    for (uint32_t k = 0; k < MOVE_PLACES; ++k) {
-        const uint32_t f = __shfl_sync(0xffffffffu, from, k), t = __shfl_sync(0xffffffffu, into, k), e = __shfl_sync(0xffffffffu, src, k);
-        moves[k] = f != PAGED_NONE;
-        s[k] = moves[k] ? paged_row(a.c, f, h, e) * elem : 0;
-        d[k] = moves[k] ? paged_row(a.to, t, h, place0 + k) * elem : 0;
-    }
-    if (vec) {
-        // 16-byte pieces of a key row, then of its value row
-        const uint32_t half = row_bytes / 16u;
-        for (uint32_t p = lane; p < 2u * half; p += 32u) {
-            const bool value = p >= half;
-            const uint32_t b = (value ? p - half : p) * 16u;
-            const unsigned char* in = value ? a.c.v : a.c.k;
-            unsigned char* out = value ? a.to.v : a.to.k;
-            uint4 x[MOVE_PLACES];
-#pragma unroll
-            for (uint32_t k = 0; k < MOVE_PLACES; ++k)
-                if (moves[k]) x[k] = *reinterpret_cast<const uint4*>(in + s[k] + b);
-#pragma unroll
-            for (uint32_t k = 0; k < MOVE_PLACES; ++k)
-                if (moves[k]) *reinterpret_cast<uint4*>(out + d[k] + b) = x[k];
+        for (uint32_t k = 0; k < MOVE_AT_ONCE; ++k) {
+            moves[k] = (mask >> (k0 + k)) & 1u;
+            s[k] = __shfl_sync(0xffffffffu, own_s, k0 + k), d[k] = __shfl_sync(0xffffffffu, own_d, k0 + k);
         }
-    } else {
+        if (vec) {
+            // 16-byte pieces of a key row, then of its value row
+            const uint32_t half = row_bytes / 16u;
+            for (uint32_t p = lane; p < 2u * half; p += 32u) {
+                const bool value = p >= half;
+                const uint32_t b = (value ? p - half : p) * 16u;
+                const unsigned char* in = value ? a.c.v : a.c.k;
+                unsigned char* out = value ? a.to.v : a.to.k;
+                uint4 x[MOVE_AT_ONCE];
 #pragma unroll
-        for (uint32_t k = 0; k < MOVE_PLACES; ++k)
-            for (uint32_t b = lane * 2u; moves[k] && b < row_bytes; b += 64u) {
-                *reinterpret_cast<uint16_t*>(a.to.k + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.k + s[k] + b);
-                *reinterpret_cast<uint16_t*>(a.to.v + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.v + s[k] + b);
+                for (uint32_t k = 0; k < MOVE_AT_ONCE; ++k)
+                    if (moves[k]) x[k] = *reinterpret_cast<const uint4*>(in + s[k] + b);
+#pragma unroll
+                for (uint32_t k = 0; k < MOVE_AT_ONCE; ++k)
+                    if (moves[k]) *reinterpret_cast<uint4*>(out + d[k] + b) = x[k];
             }
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < MOVE_AT_ONCE; ++k)
+                for (uint32_t b = lane * 2u; moves[k] && b < row_bytes; b += 64u) {
+                    *reinterpret_cast<uint16_t*>(a.to.k + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.k + s[k] + b);
+                    *reinterpret_cast<uint16_t*>(a.to.v + d[k] + b) = *reinterpret_cast<const uint16_t*>(a.c.v + s[k] + b);
+                }
+        }
     }
 }
 
