@@ -255,6 +255,27 @@ __device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t sme
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
 
+// Without a list: the place of a CTA that takes unit `unit` of row `row` as a whole, in a list of that row alone. False for a row without entries, whose zeros
+// are written. All threads of the CTA.
+template <int HD>
+__device__ __forceinline__ bool paged_direct_enter(const PagedAttnArgs& a, PagedList& s, uint32_t row, uint32_t unit, PagedPlace& p) {
+    uint32_t slot, begin, end;
+    const bool inside = paged_row_range(a, row, &slot, &begin, &end);
+    if (!inside || end <= begin) {
+        const uint32_t subgroups = (a.group + a.heads_at_once - 1u) / a.heads_at_once, kvh = unit / subgroups;
+        const uint32_t g0 = (unit - kvh * subgroups) * a.heads_at_once, G = min(a.heads_at_once, a.group - g0);
+        float* out = a.out + ((size_t)row * a.q_heads + kvh * a.group + g0) * HD;
+        for (uint32_t i = threadIdx.x; i < G * HD; i += TILES_THREADS) out[i] = 0.0f;
+        if (!inside && unit == 0 && threadIdx.x == 0) atomicOr(a.status, 1u);
+        return false;
+    }
+    if (threadIdx.x == 0) s.slot[0] = slot, s.begin[0] = begin, s.end[0] = end;
+    __syncthreads();
+    p.row = 0, p.unit = unit, p.tile = 0;
+    paged_list_enter(s, p, SPAN);
+    return true;
+}
+
 // A run of the list of work per CTA, tiles of 64 entries; a warp takes 16 of them, with a ring of its own. Against one CTA per (row, unit, 1024
 // entries): 32 rows of up to 16384 entries 198 -> 173 us, one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
 // and without a barrier per tile the warps drift apart: 187 and 179 us for the 32 rows.
@@ -270,28 +291,40 @@ struct TilesCfg {
     static constexpr int SMEM = 256 + (int)TILES_WARPS * STAGES * STAGE + (int)sizeof(PagedList);  // rings, the list
 };
 
-template <int HD, bool WIDE>
+// DIRECT, for short rows: a CTA per (row, unit) puts its warps' parts together over the rings and writes the result, without a list and a join.
+template <int HD, bool WIDE, bool DIRECT>
 __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) paged_tiles_kernel(PagedAttnArgs a) {
     using Cfg = TilesCfg<HD, WIDE>;
-    constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = Cfg::STAGES;
+    constexpr int KS = HD / 16, NT = HD / 8, CHUNKS = HD / 8, STAGES = Cfg::STAGES, ROWS = WIDE ? 16 : 8;
+    static_assert(ROWS * (HD + 2) * 4 <= STAGES * Cfg::STAGE, "a warp's part lies over its ring");
     extern __shared__ __align__(128) unsigned char smem[];
     PagedList& list = *reinterpret_cast<PagedList*>(smem + 256 + TILES_WARPS * STAGES * Cfg::STAGE);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t4 = lane & 3u;
-    const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = min(a.rows - a.row0, LIST_ROWS);
+    const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = DIRECT ? 1u : min(a.rows - a.row0, LIST_ROWS);
     pdl_wait();
     pdl_trigger();
-    if (tid < 32u) paged_list_make(a, list, rows, SPAN);
-    __syncthreads();
-    const uint64_t total = list.prefix[rows] * units;
-    const uint32_t worker = blockIdx.x, workers = ctas_at_work(total, a.workers);
-    if (worker >= workers) return;
-    const uint64_t lo = quotient(worker * total, workers);
-    const uint32_t count = (uint32_t)(quotient((worker + 1u) * total, workers) - lo);  // at least 1
-    PagedPlace at = paged_list_at(list, lo, rows, units, SPAN);
+    const uint32_t row0 = DIRECT ? blockIdx.x / units : a.row0, worker = blockIdx.x;
+    PagedPlace at;
+    uint32_t count;
+    if constexpr (DIRECT) {
+        if (!paged_direct_enter<HD>(a, list, row0, worker - row0 * units, at)) return;
+        count = at.tiles;
+    } else {
+        if (tid < 32u) paged_list_make(a, list, rows, SPAN);
+        __syncthreads();
+        const uint64_t total = list.prefix[rows] * units;
+        const uint32_t workers = ctas_at_work(total, a.workers);
+        if (worker >= workers) return;
+        const uint64_t lo = quotient(worker * total, workers);
+        count = (uint32_t)(quotient((worker + 1u) * total, workers) - lo);  // at least 1
+        at = paged_list_at(list, lo, rows, units, SPAN);
+    }
 
     // The lane copies piece `ch` of rows my_row, my_row + ROWS_AT_ONCE, ..; the swizzle of row r is r mod 8.
     constexpr uint32_t ROWS_AT_ONCE = 32u / CHUNKS, COPIES = TILE / ROWS_AT_ONCE, toSV = TILE * HD * 2u;
     const uint32_t ring = (((uint32_t)__cvta_generic_to_shared(smem) + 255u) & ~255u) + warp * (STAGES * Cfg::STAGE);  // whole rows, for the exclusive or below
+    // DIRECT: outputs [ROWS][HD], maxima and sums of warp w
+    const auto warp_part = [&](uint32_t w) { return reinterpret_cast<float*>(smem + w * (STAGES * Cfg::STAGE)); };
     const uint32_t subgroups = units / a.c.kv_heads;
     const uint32_t in_page = (1u << a.c.shift) - 1u, my_row = lane / CHUNKS, ch = lane % CHUNKS;
     const uint64_t head_bytes = (uint64_t)(HD * 2u) << a.c.shift;
@@ -360,7 +393,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             head0 = kvh * a.group + g0;
             tile_begin = at.tile;
             // A operand of the scores: rows 0-7 hi, 8-15 lo of heads 0-7; WIDE: rows are heads, hi and lo apart
-            const float* q0 = a.q + ((size_t)(a.row0 + at.row) * a.q_heads + head0 + g) * HD;
+            const float* q0 = a.q + ((size_t)(row0 + at.row) * a.q_heads + head0 + g) * HD;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -433,7 +466,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                 for (int i = 0; i < 2; ++i) {  // entries outside the row's are not read again
                     const uint32_t e = e0 + 8u * i;
                     if (g + 8u * h < G && e < a.ld_scores)
-                        *reinterpret_cast<float2*>(a.scores + ((size_t)(a.row0 + at.row) * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e) =
+                        *reinterpret_cast<float2*>(a.scores + ((size_t)(row0 + at.row) * a.q_heads + head0 + g + 8u * h) * a.ld_scores + e) =
                             make_float2(s[h][2 * i], s[h][2 * i + 1]);
                 }
         }
@@ -480,9 +513,16 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         }
         const bool ends = at.tile + 1u == at.tiles;
         if (ends || f + 1u == count) {
-            // this warp's part of the unit
-            const uint32_t row = a.row0 + at.row, kvh = at.unit / subgroups;
+            // this warp's part of the unit, for the join or (DIRECT) for this CTA
+            const uint32_t row = row0 + at.row, kvh = at.unit / subgroups;
             const size_t part = (((size_t)at.row * units + at.unit + worker) * TILES_WARPS + warp) * a.heads_at_once;
+            float* own_o = DIRECT ? warp_part(warp) : a.part_o + part * HD;
+            float* own_m = DIRECT ? own_o + ROWS * HD : a.part_m + part;
+            float* own_l = DIRECT ? own_m + ROWS : a.part_l + part;
+            if (DIRECT) {
+                cp_async_wait<0>();
+                __syncthreads();  // the rings are done with
+            }
             bool fine[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
@@ -496,8 +536,8 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                     fine[h] &= is_finite(o[n][2 * h]) & is_finite(o[n][2 * h + 1]);
                 }
                 if (g + 8u * h < G) {
-                    if (t4 == 0) a.part_m[part + g + 8 * h] = m_run[h], a.part_l[part + g + 8 * h] = l;
-                    float* dst = a.part_o + (part + g + 8 * h) * HD + 2 * t4;
+                    if (t4 == 0) own_m[g + 8 * h] = m_run[h], own_l[g + 8 * h] = l;
+                    float* dst = own_o + (g + 8 * h) * HD + 2 * t4;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
                 }
@@ -508,11 +548,31 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                 while (odd) {  // a head with something that is not finite: again, in plain f32
                     const uint32_t gh = (__ffs(odd) - 1u) / 4u, head = head0 + gh + 8u * h;
                     odd &= ~(0xfu << (4u * gh));
-                    const size_t at_part = part + gh + 8u * h, at_head = (size_t)row * a.q_heads + head;
+                    const uint32_t own = gh + 8u * h;
+                    const size_t at_head = (size_t)row * a.q_heads + head;
                     __syncwarp();
                     paged_plain_run<HD>(a, list.slot[at.row], kvh, a.q + at_head * HD, a.scores ? a.scores + at_head * a.ld_scores : nullptr,
-                                          max(at.t0, at.first + tile_begin * SPAN), min(at.t1, at.first + (at.tile + 1u) * SPAN), warp, WEIGHT_BIAS, a.part_m + at_part,
-                                          a.part_l + at_part, a.part_o + at_part * HD);
+                                          max(at.t0, at.first + tile_begin * SPAN), min(at.t1, at.first + (at.tile + 1u) * SPAN), warp, WEIGHT_BIAS, own_m + own, own_l + own,
+                                          own_o + own * HD);
+                }
+            }
+            if constexpr (DIRECT) {
+                __syncthreads();
+                for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) {
+                    const uint32_t h = i / HD, d = i % HD;
+                    float m[TILES_WARPS], M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+                    for (uint32_t w = 0; w < TILES_WARPS; ++w) m[w] = warp_part(w)[ROWS * HD + h], M = fmaxf(M, m[w]);
+#pragma unroll
+                    for (uint32_t w = 0; w < TILES_WARPS; ++w) {
+                        const float l = warp_part(w)[ROWS * HD + ROWS + h];
+                        const float e = l != 0.0f ? (m[w] == -INFINITY ? 1.0f : exp2f(m[w] - M)) : 0.0f;  // a sum without a maximum: NaN, as it is
+                        L += l * e;
+                        if (e != 0.0f) O = fmaf(e, warp_part(w)[h * HD + d], O);
+                    }
+                    const size_t head = (size_t)row * a.q_heads + head0 + h;
+                    a.out[head * HD + d] = L == 0.0f ? 0.0f : O / L;
+                    if (a.stat && d == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
                 }
             }
         }
@@ -728,12 +788,18 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
 // Whether a CTA per head and row leaves most of the device idle.
 bool few_heads(const M40llmCudaContext* ctx, uint32_t q_heads, uint32_t rows) { return (uint64_t)q_heads * rows <= 2ull * (uint64_t)ctx->sm_count; }
 
-template <int HD, bool WIDE>
+template <int HD, bool WIDE, bool DIRECT>
 cudaError_t launch_tiles(M40llmCudaContext* ctx, const PagedAttnArgs& a) {
     using Cfg = TilesCfg<HD, WIDE>;
-    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
     if (e != cudaSuccess) return e;
-    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
+    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE, DIRECT>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
+}
+template <bool DIRECT>
+cudaError_t launch_tiles_of(M40llmCudaContext* ctx, const PagedAttnArgs& a) {
+    const bool wide = a.heads_at_once > 8u;
+    if (a.c.hd == 64u) return wide ? launch_tiles<64, true, DIRECT>(ctx, a) : launch_tiles<64, false, DIRECT>(ctx, a);
+    return wide ? launch_tiles<128, true, DIRECT>(ctx, a) : launch_tiles<128, false, DIRECT>(ctx, a);
 }
 
 // All rows in launches of up to 256, each followed by its join. `ctas`: how many are resident, `span`: entries of a tile of the list.
@@ -814,11 +880,14 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         a.splits = (uint32_t)((a.bound + chunk - 1) / chunk);
     }
     const size_t heads = (size_t)c->rows * c->q_heads;
-    if (list || a.splits > 1 || c->weights_out) {
+    const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
+    // Short rows: a CTA takes a unit as a whole. One row of 64 entries, 32 / 4 heads of 64: 4.3 us against 6.8, of 500 9.8 against 7.2; 8 rows of up to 500,
+    // 32 / 8 heads of 128: 12.0 against 13.7, 48 rows 24.8 against 28.1, of 1000 alike. (In paged_lanes_kernel it was slower: 9.8 us against 8.5.)
+    const bool direct = tiles && a.bound <= (c->rows * units >= 64u ? 512u : 256u) && c->rows * units <= 0x7fffffffu;
+    if ((list && !direct) || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? (a.bound + 3u) & ~3u : 0u;
         const size_t rows_at_once = c->rows < LIST_ROWS ? c->rows : LIST_ROWS;
-        const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
-        const size_t parts = list ? (rows_at_once * units + ctas) * a.part_warps * a.heads_at_once : heads * a.splits;
+        const size_t parts = direct ? 0 : (list ? (rows_at_once * units + ctas) * a.part_warps * a.heads_at_once : heads * a.splits);
         const size_t floats = parts * (hd + 2) + heads * 2 + 4 + heads * (size_t)a.ld_scores;
         const size_t prefix = (LIST_ROWS + 1) * sizeof(uint64_t);  // first, for its alignment; 16 bytes more keep the outputs' rows aligned
         unsigned char* work_area = (unsigned char*)m40_ensure_scratch(ctx, 1, prefix + 8 + floats * sizeof(float), 0);
@@ -833,12 +902,12 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         }
     }
     cudaError_t e;
-    if (tiles) {
-        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) {
-            const bool wide = x.heads_at_once > 8u;
-            return hd == 64u ? (wide ? launch_tiles<64, true>(ctx, x) : launch_tiles<64, false>(ctx, x))
-                             : (wide ? launch_tiles<128, true>(ctx, x) : launch_tiles<128, false>(ctx, x));
-        });
+    if (direct) {
+        a.workers = (uint32_t)(c->rows * units);
+        e = launch_tiles_of<true>(ctx, a);
+        M40_COUNT_LAUNCH(ctx);
+    } else if (tiles) {
+        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x); });
     } else if (by_lanes) {
         e = launch_list(ctx, a, ctas, 8u * lanes.warps, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
     } else {

@@ -114,9 +114,10 @@ SHAPES = [(8, 2, 64, 16), (4, 4, 128, 32), (7, 1, 128, 1), (10, 2, 64, 2), (9, 1
 
 @pytest.mark.parametrize("kind", ["f16", "f32"])
 @pytest.mark.parametrize("q_heads,kv_heads,dim,page", SHAPES)
-def test_attention_shapes(nat, kind, q_heads, kv_heads, dim, page):
+@pytest.mark.parametrize("entries", [200, 300])
+def test_attention_shapes(nat, kind, q_heads, kv_heads, dim, page, entries):
     rng = np.random.default_rng(q_heads * 1000 + dim + page)
-    c = T.Cache(nat, rng, len(LENS), 200, kv_heads, dim, page, kind)
+    c = T.Cache(nat, rng, len(LENS), entries, kv_heads, dim, page, kind)
     q = (2 * rng.standard_normal((len(LENS), q_heads, dim))).astype(np.float32)
     slot = rng.permutation(len(LENS))
     got, _ = T.attend(nat, c, q, slot, LENS)
@@ -145,8 +146,9 @@ def test_attention_window(nat, kind, dim, heads):
     assert not got[3].any() and not got[4].any() and not got[6].any() and T.status(nat) == 0
 
 
-@pytest.mark.parametrize("kind,dim,offset", [("f16", 128, 0), ("f16", 64, 0), ("f16", 64, 1), ("f32", 64, 0), ("f32", 64, 1), ("f16", 36, 0)])
-def test_attention_ignores_what_is_masked(nat, kind, dim, offset):
+@pytest.mark.parametrize("kind,dim,offset", [("f16", 128, 0), ("f16", 64, 0), ("f16", 64, 1), ("f32", 64, 0), ("f32", 64, 1), ("f16", 36, 0), ("f16", 96, 0)])
+@pytest.mark.parametrize("max_len", [0, 200])
+def test_attention_ignores_what_is_masked(nat, kind, dim, offset, max_len):
     """Infinities and NaN behind a row's entries, before its window, on its last page and on other pages do not reach the output."""
     rng = np.random.default_rng(dim + offset)
     c = T.Cache(nat, rng, 4, 300, 2, dim, 16, kind, offset=offset)
@@ -160,24 +162,25 @@ def test_attention_ignores_what_is_masked(nat, kind, dim, offset):
     for pool in (c.k, c.v):
         pool.transpose(0, 2, 1, 3)[~seen] = rng.choice(bad, pool.transpose(0, 2, 1, 3)[~seen].shape)
     c.upload()
-    got, _ = T.attend(nat, c, q, [0, 1, 2, 3], length, begin=begin)
+    got, _ = T.attend(nat, c, q, [0, 1, 2, 3], length, begin=begin, max_len=max_len)
     T.check_attention(c, q, [0, 1, 2, 3], length, got, begin=begin)
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 128), ("f32", 128)])
-def test_attention_values_that_are_not_finite(nat, kind, dim):
+@pytest.mark.parametrize("n", [300, 230])
+def test_attention_values_that_are_not_finite(nat, kind, dim, n):
     """What a row does see reaches its output as the formula says; the rows beside it keep theirs."""
     rng = np.random.default_rng(1)
-    c = T.Cache(nat, rng, 3, 300, 1, dim, 16, kind)
+    c = T.Cache(nat, rng, 3, n, 1, dim, 16, kind)
     at = lambda s, e: (c.table[s, e // 16], 0, e % 16)  # noqa: E731
     c.v[at(0, 5)][3] = np.inf
     c.k[at(1, 200)][0] = np.nan
     c.upload()
     q = rng.standard_normal((3, 4, dim)).astype(np.float32)
-    got, _ = T.attend(nat, c, q, [0, 1, 2], [300, 300, 300])
+    got, _ = T.attend(nat, c, q, [0, 1, 2], [n, n, n])
     assert (got[0][:, 3] == np.inf).all() and np.isfinite(np.delete(got[0], 3, 1)).all()
     assert np.isnan(got[1]).all()
-    T.check_attention(c, q[2:], [2], [300], got[2:])
+    T.check_attention(c, q[2:], [2], [n], got[2:])
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 128), ("f16", 64), ("f32", 40)])
@@ -217,6 +220,18 @@ def test_attention_rows_share_slots_and_pages(nat):
     q = rng.standard_normal((4, 8, 64)).astype(np.float32)
     got, _ = T.attend(nat, c, q, [0, 1, 1, 0], [200, 201, 202, 80])
     T.check_attention(c, q, [0, 1, 1, 0], [200, 201, 202, 80], got)
+
+
+@pytest.mark.parametrize("kind,dim,heads,kv_heads", [("f16", 128, 8, 2), ("f16", 64, 32, 2), ("f32", 64, 4, 4), ("f16", 72, 6, 2), ("f16", 64, 20, 1)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_attention_weights_of_short_rows(nat, kind, dim, heads, kv_heads, in_place):
+    rng = np.random.default_rng(dim + heads)
+    c = T.Cache(nat, rng, 5, 240, kv_heads, dim, 16, kind)
+    w = rng.random((5, kv_heads, c.capacity)).astype(np.float32)
+    slot, length, begin = [3, 1, 3, 0, 3, 4], [200, 130, 201, 0, 100, 1], [0, 10, 0, 0, 64, 0]
+    q = (2 * rng.standard_normal((6, heads, dim))).astype(np.float32)
+    got, gw = T.attend(nat, c, q, slot, length, begin=begin, weights=w, ld=c.capacity, in_place=in_place)
+    T.check_attention(c, q, slot, length, got, begin=begin, weights=w, got_w=gw, before=w if in_place else np.full(w.shape, -5.0, np.float32))
 
 
 @pytest.mark.parametrize("kind,dim,heads,kv_heads", [("f16", 128, 8, 2), ("f16", 64, 32, 2), ("f32", 64, 4, 4), ("f16", 72, 6, 2), ("f16", 64, 20, 1)])
