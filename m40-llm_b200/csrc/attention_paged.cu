@@ -705,27 +705,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
 // Bound by the scores, which mostly come out of L2.
 constexpr uint32_t WEIGHTS_AT_ONCE = 1024;
 __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uint32_t vec) {
-    __shared__ uint32_t s_most, s_count, s_row[256];
     pdl_wait();
     pdl_trigger();
-    const uint32_t tid = threadIdx.x, row = blockIdx.z, h = blockIdx.y;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, row = blockIdx.z, h = blockIdx.y;
     const uint32_t slot = a.row_slot[row];
     if (slot >= a.c.slots) return;
-    if (tid == 0) s_most = 0u, s_count = 0u;
-    __syncthreads();
+    // every warp looks at all rows, 32 at a time, a lane each
+    uint32_t s, b, n, most = 0;
     bool skip = false;
-    uint32_t most = 0;
-    for (uint32_t r = tid; r < a.rows; r += 256u) {
-        uint32_t s, b, n;
-        const bool inside = paged_row_range(a, r, &s, &b, &n);
-        if (s != slot) continue;
-        if (r < row || !inside) skip = true;
-        most = max(most, n);
+    for (uint32_t r0 = 0; r0 < a.rows; r0 += 32u) {
+        const uint32_t r = r0 + lane;
+        const bool inside = r < a.rows && paged_row_range(a, r, &s, &b, &n), mine = r < a.rows && s == slot;
+        if (mine) skip |= r < row || !inside, most = max(most, n);
     }
+    if (__any_sync(0xffffffffu, skip)) return;
     most = __reduce_max_sync(0xffffffffu, most);
-    if ((tid & 31u) == 0 && most) atomicMax(&s_most, most);
-    if (__syncthreads_or(skip)) return;
-    most = s_most;
     const uint32_t e = blockIdx.x * WEIGHTS_AT_ONCE + 4u * tid;
     if (blockIdx.x * WEIGHTS_AT_ONCE >= most) return;
     const size_t at = ((size_t)slot * a.c.kv_heads + h) * a.ld_weights + e;
@@ -738,26 +732,16 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) w[i] = a.weights_in && e + i < most ? a.weights_in[at + i] : 0.0f;
     }
-    for (uint32_t r0 = row; r0 < a.rows; r0 += 256u) {  // the slot's rows among the next 256, in order
-        const uint32_t r = r0 + tid, mine = r < a.rows && a.row_slot[r] == slot ? 1u : 0u;
-        __syncthreads();
-        if (tid == 0) s_count = 0u;
-        const uint32_t mask = __ballot_sync(0xffffffffu, mine);
-        for (uint32_t k = 0; k < 8u; ++k) {
-            __syncthreads();
-            if (tid / 32u == k && mask) {
-                if (mine) s_row[s_count + __popc(mask & ((1u << (tid & 31u)) - 1u))] = r;
-                __syncwarp();
-                if ((tid & 31u) == 0) s_count += __popc(mask);
-            }
-        }
-        __syncthreads();
-        for (uint32_t k = 0; k < s_count; ++k) {
-            uint32_t s, b, n;
-            paged_row_range(a, s_row[k], &s, &b, &n);
+    for (uint32_t r0 = row & ~31u; r0 < a.rows; r0 += 32u) {
+        const uint32_t r = r0 + lane;
+        if (a.rows > 32u && r < a.rows) paged_row_range(a, r, &s, &b, &n);  // up to 32 are there already
+        uint32_t mask = __ballot_sync(0xffffffffu, r < a.rows && s == slot);
+        while (mask) {  // the slot's rows in order
+            const uint32_t k = __ffs(mask) - 1u, from = __shfl_sync(0xffffffffu, b, k), to = __shfl_sync(0xffffffffu, n, k);
+            mask &= mask - 1u;
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const size_t head = (size_t)s_row[k] * a.q_heads + h * a.group;
-            const bool all = whole && e >= b && e + 4u <= n;
+            const size_t head = (size_t)(r0 + k) * a.q_heads + h * a.group;
+            const bool all = whole && e >= from && e + 4u <= to;
 #pragma unroll 4
             for (uint32_t g = 0; g < a.group; ++g) {
                 const float M = a.stat[2 * (head + g)], inv = a.stat[2 * (head + g) + 1];
@@ -769,7 +753,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
                 } else {
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i)
-                        if (e + i >= b && e + i < n) sum[i] += exp2f(sc[i] - M) * inv;
+                        if (e + i >= from && e + i < to) sum[i] += exp2f(sc[i] - M) * inv;
                 }
             }
 #pragma unroll
