@@ -768,7 +768,8 @@ int m40llm_paged_append_async(M40llmCudaContext* ctx, const M40llmPagedCache* ca
  * work is dealt by (0: the capacity; a row beyond it is one outside the cache).
  * With weights_out f32 [slots][kv_heads][ld_weights]: entry e of a slot that has rows in the call, e below the largest row_len of
  * these, gets weights_in[...][e] (null: 0; may be weights_out itself) + the softmax weights that these rows gave it, summed over the q heads of its kv
- * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. */
+ * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. The scores are kept until the sums are known:
+ * about rows * q_heads * max_len floats of scratch, so max_len should be given. */
 typedef struct {
     const void* q;
     void* out;
