@@ -768,7 +768,7 @@ int m40llm_paged_append_async(M40llmCudaContext* ctx, const M40llmPagedCache* ca
  * work is dealt by (0: the capacity; a row beyond it is one outside the cache).
  * With weights_out f32 [slots][kv_heads][ld_weights]: entry e of a slot that has rows in the call, e below the largest row_len of
  * these, gets weights_in[...][e] (null: 0; may be weights_out itself) + the softmax weights that these rows gave it, summed over the q heads of its kv
- * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. The scores are kept until the sums are known:
+ * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. Where all of a row's scores are -inf, it gives zeros and no weight. The scores are kept until the sums are known:
  * about rows * q_heads * max_len floats of scratch, so max_len should be given. */
 typedef struct {
     const void* q;
@@ -788,7 +788,7 @@ int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llmPagedCache*
  * weight (NaN below all else); the lower entry first where that leaves a choice. Kept entries below the new length stay where they are; the
  * places of the others there are taken, in ascending order, by the kept ones from behind the new end. origin u32 [count][kv_heads][keep] (or null) says where each entry came from (0xffffffff beyond the new length),
  * new_len u32 [count] = min(len, keep). `to` null: in place, only what moves is copied; it may hold pages that no other slot
- * reads. Otherwise the kept entries go to the same slots of `to`, a cache of the same heads, size and type on other pages. weights_out and
+ * reads. Otherwise the kept entries go to the same slots of `to`, a cache of the same heads, size and type on other pages. new_len may be len. weights_out and
  * entry_pos_out [slots][kv_heads][ld] take the kept entries' values (null: not kept; the arrays themselves: in place).
  * max_len bounds len (0: the capacity). A slot outside the cache or named before in seq, or a length beyond max_len, keeps nothing: new_len 0. */
 typedef struct {

@@ -280,7 +280,8 @@ __device__ __forceinline__ bool paged_direct_enter(const PagedAttnArgs& a, Paged
 // entries): 32 rows of up to 16384 entries 198 -> 173 us, one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
 // and without a barrier per tile the warps drift apart: 187 and 179 us for the 32 rows.
 //   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units.
-//   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them. A group has
+//   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them; a head's query is
+//                         brought to 2^9 .. 2^10 by a power of two first (its largest value), as the lo of a small value would lose its bits. A group has
 //                         at most 8 heads as a rule: hi and lo are then the two halves of the 16 rows of ONE operand, and the halves of the result are
 //                         added (WIDE: two products).
 //   softmax               online in base 2; the outputs are rescaled only when a maximum moved.
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     const uint32_t v_at = ring + toSV + vr * (HD * 2u) + (((mj >> 1) ^ (vr & 7u)) * 16u);
     constexpr int H = WIDE ? 2 : 1;  // heads of a thread
     uint32_t qa[KS][4], qb[WIDE ? KS : 1][4];
-    float o[NT][4], m_run[H], l_run[H];
+    float o[NT][4], m_run[H], l_run[H], down[H];  // scores are multiplied by down
     uint32_t head0 = 0, G = 0, tile_begin = 0;
     bool entering = true;
     for (uint32_t f = 0; f < count; ++f) {
@@ -393,24 +394,31 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             head0 = kvh * a.group + g0;
             tile_begin = at.tile;
             // A operand of the scores: rows 0-7 hi, 8-15 lo of heads 0-7; WIDE: rows are heads, hi and lo apart
-            const float* q0 = a.q + ((size_t)(row0 + at.row) * a.q_heads + head0 + g) * HD;
+            const float* q0 = a.q + ((size_t)(row0 + at.row) * a.q_heads + head0 + g) * HD + 2 * t4;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int h = 0; h < H; ++h) {
+                float2 x[KS][2];
+                float big = 0.0f;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t k0 = ks * 16 + half * 8 + 2 * t4;
-                    const float2 x = g < G ? *reinterpret_cast<const float2*>(q0 + k0) : make_float2(0.0f, 0.0f);
-                    uint32_t hi, lo_part;
-                    split_h2(x.x * a.scale, x.y * a.scale, &hi, &lo_part);
-                    qa[ks][2 * half] = hi;
-                    if (WIDE) {
-                        qb[ks][2 * half] = lo_part;
-                        const float2 y = g + 8u < G ? *reinterpret_cast<const float2*>(q0 + 8 * HD + k0) : make_float2(0.0f, 0.0f);
-                        split_h2(y.x * a.scale, y.y * a.scale, &qa[ks][2 * half + 1], &qb[ks][2 * half + 1]);
-                    } else {
-                        qa[ks][2 * half + 1] = lo_part;
-                    }
+                for (int i = 0; i < 2 * KS; ++i) {
+                    float2& y = x[i / 2][i % 2];
+                    y = g + 8u * h < G ? *reinterpret_cast<const float2*>(q0 + 8 * HD * h + 8 * i) : make_float2(0.0f, 0.0f);
+                    y.x *= a.scale, y.y *= a.scale;
+                    big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
                 }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const uint32_t up = min(263u - (__float_as_uint(big) >> 23), 247u);
+                const float factor = __uint_as_float(up << 23);
+                down[h] = __uint_as_float((254u - up) << 23);
+#pragma unroll
+                for (int i = 0; i < 2 * KS; ++i) {
+                    const float2 y = x[i / 2][i % 2];
+                    const int at_a = 2 * (i % 2) + (WIDE ? h : 0);
+                    uint32_t* lo_at = WIDE ? &qb[WIDE ? i / 2 : 0][at_a] : &qa[i / 2][at_a + 1];
+                    split_h2(y.x * factor, y.y * factor, &qa[i / 2][at_a], lo_at);
+                }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 #pragma unroll
@@ -447,6 +455,8 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         for (int h = 0; h < H; ++h) {
             s[h][0] = WIDE ? s0[0][2 * h] : s0[0][0] + s0[0][2], s[h][1] = WIDE ? s0[0][2 * h + 1] : s0[0][1] + s0[0][3];
             s[h][2] = WIDE ? s1[0][2 * h] : s1[0][0] + s1[0][2], s[h][3] = WIDE ? s1[0][2 * h + 1] : s1[0][1] + s1[0][3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[h][i] *= down[h];
         }
         if (base < at.t0 || base + TILE > at.t1 || __any_sync(0xffffffffu, bad)) {
             const uint32_t* own_pages = a.c.table + (size_t)list.slot[at.row] * a.c.max_pages;
@@ -572,7 +582,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                     }
                     const size_t head = (size_t)row * a.q_heads + head0 + h;
                     a.out[head * HD + d] = L == 0.0f ? 0.0f : O / L;
-                    if (a.stat && d == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+                    if (a.stat && d == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
                 }
             }
         }
@@ -636,7 +646,7 @@ __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t 
     L = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) L += red[8 + i];
-    if (a.stat && tid == 0 && blockIdx.z == 0) a.stat[2 * head] = M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+    if (a.stat && tid == 0 && blockIdx.z == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
@@ -810,10 +820,8 @@ cudaError_t launch_rows(const PagedAttnArgs& a, dim3 grid, uint32_t T, uint32_t 
     const uint32_t dv = (a.c.hd + ROWS_THREADS - 1) / ROWS_THREADS;
     void (*kernel)(PagedAttnArgs, uint32_t, uint32_t, uint32_t) =
         dv == 1 ? paged_rows_kernel<ET, GT, 1> : (dv == 2 ? paged_rows_kernel<ET, GT, 2> : paged_rows_kernel<ET, GT, 4>);
-    if (smem > 48u * 1024u) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PAGED_SMEM_MOST);  // the same from every thread
+    if (e != cudaSuccess) return e;
     return m40_launch_dependent(kernel, grid, dim3(ROWS_THREADS), smem, s, a, T, vec, pitch);
 }
 

@@ -39,6 +39,7 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gm
 // entries (from the multiple of span that the row's first entry lies behind). Every resident CTA takes an equal run of the list, so that none starts late and none
 // ends early, whatever the lengths. Each warp leaves a part (maximum, sum, output) of every unit that its CTA's run touches, and paged_join_kernel puts the
 // parts together: CTA c has part number u + c in unit u of all units, which no other has, as c or u grows from one part of the list to the next.
+constexpr uint32_t PAGED_SMEM_MOST = 216u * 1024u;  // dynamic shared memory that the kernels are allowed, whatever a call takes
 constexpr uint32_t LIST_ROWS = 256;  // rows of a launch: their ranges stay in shared memory
 
 // The CTA whose run holds tile x of `total`; CTA i of n has [i total / n, (i + 1) total / n).

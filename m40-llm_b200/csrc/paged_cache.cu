@@ -177,6 +177,7 @@ struct EvictArgs {
     uint32_t* new_len;  // [count]
     uint32_t* plan;     // scratch [count][kv_heads][keep]: a place's own entry, EVICT_HOLE + the hole's number, or PAGED_NONE beyond the new length
     uint32_t* late;     // scratch, likewise: kept entries behind the new end, in order
+    uint32_t* kept;     // scratch [count]: the new lengths, which the copy gives out, as new_len may be the lengths that every CTA reads
     uint32_t* status;
     uint32_t keep, first, recent, ld, bound, in_place;
     uint32_t cached;    // entries that a CTA's shared memory holds
@@ -252,7 +253,7 @@ __device__ __forceinline__ uint32_t lanes_before(uint32_t own) {
 // out by itself (else two more histograms follow). Then the entries are counted once, larger and equal ones below and behind the new end, which gives every
 // warp the numbers of its ties, holes and kept entries behind the end, so that the plan is written without an order of who comes first. What CTAs tell each other
 // is stored into the others' memory before a barrier: loads from there took 400 cycles each. Against one CTA and four passes from memory: 4 x 8 heads
-// of 8192 entries with the copy 76 -> 24 us, 8 heads of 32768 217 -> 28.5. Bound by the barriers of the cluster and a chain of short steps.
+// of 8192 entries with the copy 76 -> 23.1 us, 8 heads of 32768 217 -> 27.1. Bound by the barriers of the cluster and a chain of short steps.
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs a) {
     extern __shared__ __align__(16) uint32_t s_dyn[];  // [cached] keys, [cached] positions
     __shared__ SelectShared sh;
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     uint32_t* plan = a.plan + ((size_t)i * a.c.kv_heads + h) * a.keep;
     const uint32_t kept = bad ? 0u : min(len, a.keep);
     if (tid == 0 && h == 0 && me == 0) {
-        a.new_len[i] = kept;
+        a.kept[i] = kept;
         if (bad) atomicOr(a.status, 1u);
     }
     const uint32_t all = me * SELECT_THREADS + tid, step = peers * SELECT_THREADS;
@@ -287,6 +288,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictArgs 
     const bool cached = per <= a.cached;
     uint32_t* s_key = s_dyn;
     uint32_t* s_pos = s_dyn + a.cached;
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // every CTA of the cluster is there before anything is stored into it
     uint32_t newest = 0;
     if (pos) {
@@ -486,6 +488,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t r
     const uint32_t i = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31u, place0 = (blockIdx.x * 8u + (threadIdx.x >> 5)) * MOVE_PLACES;
     if (place0 >= a.keep) return;
     const uint32_t slot = a.seq[i];
+    if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.new_len[i] = a.kept[i];
     const size_t list = ((size_t)i * a.c.kv_heads + h) * a.keep, base = ((size_t)slot * a.c.kv_heads + h) * a.ld;
     // lanes 0 .. MOVE_PLACES - 1 look a place up each
     uint32_t src = PAGED_NONE, from = PAGED_NONE, into = PAGED_NONE;
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a, uint32_t r
 }
 
 cudaError_t launch_select(const EvictArgs& a, uint32_t count, uint32_t peers, size_t smem, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(SELECT_CACHED * 8u));  // the same from every thread
     if (e == cudaSuccess && peers > 8u) e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -582,6 +585,7 @@ int m40llm_paged_append_async(M40llmCudaContext* ctx, const M40llmPagedCache* ca
     const uint64_t wide = (uint64_t)c->q_heads * cache->head_dim, tight = (uint64_t)cache->kv_heads * cache->head_dim;
     if (wide > 0xffffffffull || tight > 0xffffffffull || 2ull * c->pairs > cache->head_dim || c->rope_layout > 1u) return -2;
     if (c->ld && (c->ld < wide || c->ld < tight)) return -2;
+    if (c->q_heads && c->q_out == c->q && c->ld && c->ld != wide) return -2;
     if ((c->entry_pos || c->weights) && c->ld_entry < paged_capacity(a.c)) return -2;
     if (m40_ensure_device(ctx) != 0) return -1;
     a.q = (const float*)c->q;
@@ -630,6 +634,7 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     if (c->count == 0 || c->keep == 0 || c->keep > capacity || c->keep > paged_capacity(a.to)) return -2;
     if ((uint64_t)c->first + c->recent > c->keep || c->ld < capacity || c->max_len > capacity) return -2;
     if (to->kv_heads != cache->kv_heads || to->head_dim != cache->head_dim || to->slots < cache->slots) return -2;
+    if (to->k == cache->k && to->table == cache->table && (to->v != cache->v || to->page_tokens != cache->page_tokens || to->max_pages != cache->max_pages)) return -2;
     if (to->elem_dtype != cache->elem_dtype) return -4;
     if (c->count > 65535u) return M40LLM_ERR_LIMIT;
     if (m40_ensure_device(ctx) != 0) return -1;
@@ -649,10 +654,11 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     a.ld = c->ld;
     a.bound = c->max_len ? c->max_len : capacity;
     const size_t places = (size_t)c->count * cache->kv_heads * c->keep;
-    uint32_t* work = (uint32_t*)m40_ensure_scratch(ctx, 1, 2 * places * sizeof(uint32_t), 0);
+    uint32_t* work = (uint32_t*)m40_ensure_scratch(ctx, 1, (2 * places + c->count) * sizeof(uint32_t), 0);
     if (!work) return -5;
     a.plan = work;
     a.late = work + places;
+    a.kept = work + 2 * places;
     a.origin = c->origin;
     // as many CTAs for a list as fill the device once, with 512 entries or more each
     const uint64_t lists = (uint64_t)c->count * cache->kv_heads;

@@ -193,6 +193,36 @@ def test_attention_large_and_small_scores(nat, kind, dim):
     T.check_attention(c, q, [0, 1], [600, 600], got)
 
 
+@pytest.mark.parametrize("kind,dim,heads", [("f16", 128, 8), ("f16", 64, 12), ("f32", 64, 8), ("f16", 40, 8)])
+@pytest.mark.parametrize("queries,keys", [(1e-5, 4096.0), (1e-12, 8192.0), (1e6, 1e-3)])
+def test_attention_sizes_of_queries_and_keys(nat, kind, dim, heads, queries, keys):
+    """Queries far from 1 keep their bits: the scores are what they are for queries and keys that share the size."""
+    rng = np.random.default_rng(3)
+    c = T.Cache(nat, rng, 2, 600, 1, dim, 16, kind)
+    c.k = (c.k.astype(np.float32) * np.float32(keys)).astype(c.dtype)
+    c.upload()
+    q = (queries * rng.standard_normal((2, heads, dim))).astype(np.float32)
+    got, _ = T.attend(nat, c, q, [0, 1], [600, 130])
+    T.check_attention(c, q, [0, 1], [600, 130], got)
+
+
+@pytest.mark.parametrize("kind,dim", [("f16", 128), ("f32", 64), ("f16", 20)])
+@pytest.mark.parametrize("n", [100, 700])
+def test_attention_weights_where_nothing_is_seen(nat, kind, dim, n):
+    """Rows whose pages are all outside the pool, and rows whose scores are all -inf: zeros, and the weights stay."""
+    rng = np.random.default_rng(4)
+    c = T.Cache(nat, rng, 3, n, 1, dim, 16, kind)
+    c.table[1] = 0xffffffff
+    for page in c.table[2]:
+        c.k[page] = -np.inf
+    c.upload()
+    w = rng.random((3, 1, c.capacity)).astype(np.float32)
+    q = np.abs(rng.standard_normal((3, 2, dim))).astype(np.float32) + np.float32(0.1)
+    got, gw = T.attend(nat, c, q, [0, 1, 2], [n, n, n], weights=w, ld=c.capacity)
+    assert not got[1].any() and not got[2].any() and np.array_equal(gw[1:, :, :n], w[1:, :, :n]) and T.status(nat) == 1
+    T.check_attention(c, q[:1], [0], [n], got[:1])
+
+
 @pytest.mark.parametrize("kind,dim", [("f16", 128), ("f16", 64), ("f32", 64), ("f16", 20)])
 def test_attention_outside(nat, kind, dim):
     """Rows outside the cache give zeros and status bit 1; entries on a page outside the pool are masked."""
@@ -470,6 +500,29 @@ def test_evict_without_origins_in_place_twice(nat):
     c.k, c.v = c.download()
     got2 = run_evict(nat, c, [1], [50], 50, 2, 10, got[2], None, in_place=True, origin=False)
     assert np.array_equal(got2[2], got[2]) and all(np.array_equal(a, b) for a, b in zip(c.download(), (c.k, c.v)))
+
+
+@pytest.mark.parametrize("n", [5000, 300])
+def test_evict_lengths_in_place(nat, n):
+    """new_len may be the array of the lengths."""
+    rng = np.random.default_rng(12)
+    c = T.Cache(nat, rng, 3, n, 2, 64, 16)
+    keep, length = 200, [n, 150, n - 7]
+    w = rng.random((3, 2, c.capacity)).astype(np.float32)
+    d_len, d_w = T.u32(nat, length), T.f32(nat, w)
+    origin = T.u32(nat, np.zeros((3, 2, keep)))
+    call = N.PagedEvict(seq=T.u32(nat, [0, 1, 2]).ptr, len=d_len.ptr, weights=d_w.ptr, weights_out=d_w.ptr, origin=origin.ptr, new_len=d_len.ptr, count=3,
+                        keep=keep, ld=c.capacity)
+    desc = c.desc()
+    assert nat.lib.m40llm_paged_evict_async(nat.ctx, C.byref(desc), C.byref(call)) == 0
+    nat.sync(1)
+    assert d_len.download(np.uint32, 3).tolist() == [200, 150, 200] and T.status(nat) == 0
+    got = origin.download(np.uint32, (3, 2, keep))
+    for i in range(3):
+        m = min(length[i], keep)
+        for h in range(2):
+            best = np.argsort(-w[i, h, :length[i]], kind="stable")[:m]
+            assert np.array_equal(np.sort(got[i, h, :m]), np.sort(best)) and (got[i, h, m:] == 0xffffffff).all()
 
 
 def test_evict_outside(nat):

@@ -102,3 +102,15 @@ def test_null_handles(pkg):
     assert L.m40llm_paged_evict_async(CTX, None, None) == -1
     assert L.m40llm_logprobs_f32_async(None, C.byref(logprobs())) == -1
     assert L.m40llm_logprobs_f32_async(CTX, None) == -1
+
+
+def test_queries_in_place_of_a_packed_projection(pkg):
+    """The turned queries are packed rows, so they may take the place of their input only where that is packed too."""
+    L = pkg.native.lib()
+    assert L.m40llm_paged_append_async(CTX, C.byref(cache()), C.byref(append(ld=8 * 64 + 4, q_out=P))) == -2
+
+
+@pytest.mark.parametrize("change", [dict(page_tokens=32), dict(max_pages=1), dict(v=2 * P)])
+def test_eviction_into_another_view_of_the_same_pages(pkg, change):
+    L, to = pkg.native.lib(), cache(**change)
+    assert L.m40llm_paged_evict_async(CTX, C.byref(cache()), C.byref(evict(to=C.addressof(to)))) == -2
