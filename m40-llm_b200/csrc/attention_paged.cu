@@ -8,6 +8,7 @@
 //   paged_rows_kernel   what is left, odd head sizes and alignments: f32 multiply-adds on tiles in shared memory
 #include "attention_paged.cuh"
 #include "stack_math.cuh"
+#include "tc_ptx.cuh"
 
 namespace {
 
@@ -255,7 +256,7 @@ __device__ __forceinline__ void ldmatrix_trans_at(uint32_t (&r)[4], uint32_t sme
 // rounded, is what a part carries as its maximum.
 constexpr float WEIGHT_BIAS = 15.0f;
 
-// Without a list: the place of a CTA that takes unit `unit` of row `row` as a whole, in a list of that row alone. False for a row without entries, whose zeros
+// Without a list: the place of a CTA that takes unit `unit` of row `row` from its first tile on, in a list of that row alone. False for a row without entries, whose zeros
 // are written. All threads of the CTA.
 template <int HD>
 __device__ __forceinline__ bool paged_direct_enter(const PagedAttnArgs& a, PagedList& s, uint32_t row, uint32_t unit, PagedPlace& p) {
@@ -276,6 +277,8 @@ __device__ __forceinline__ bool paged_direct_enter(const PagedAttnArgs& a, Paged
     return true;
 }
 
+constexpr uint32_t DIRECT_CLUSTER = 8;
+
 // A run of the list of work per CTA, tiles of 64 entries; a warp takes 16 of them, with a ring of its own. Against one CTA per (row, unit, 1024
 // entries): 32 rows of up to 16384 entries 198 -> 173 us, one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
 // and without a barrier per tile the warps drift apart: 187 and 179 us for the 32 rows.
@@ -290,9 +293,12 @@ struct TilesCfg {
     static constexpr int STAGES = HD == 128 ? 3 : 4, CTAS = HD == 128 ? 2 : 3;
     static constexpr int STAGE = 2 * (int)TILE * HD * 2;                                                                    // K and V of a tile
     static constexpr int SMEM = 256 + (int)TILES_WARPS * STAGES * STAGE + (int)sizeof(PagedList);  // rings, the list
+    // DIRECT: what the CTAs of a cluster tell each other, by the teller's number: maxima and sums of the heads, outputs of the reader's share of the dimensions
+    static constexpr int HEADS = WIDE ? 16 : 8, TOLD = (2 * (int)DIRECT_CLUSTER * HEADS + HEADS * HD) * 4;
 };
 
-// DIRECT, for short rows: a CTA per (row, unit) puts its warps' parts together over the rings and writes the result, without a list and a join.
+// DIRECT, for short rows: a CTA per (row, unit), or a cluster of them with an equal share of the tiles each, puts its warps' parts together over the rings and writes the
+// result, without a list and a join. In a cluster the CTAs store their parts into the memory of the one that puts the dimensions together.
 template <int HD, bool WIDE, bool DIRECT>
 __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) paged_tiles_kernel(PagedAttnArgs a) {
     using Cfg = TilesCfg<HD, WIDE>;
@@ -304,12 +310,17 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), rows = DIRECT ? 1u : min(a.rows - a.row0, LIST_ROWS);
     pdl_wait();
     pdl_trigger();
-    const uint32_t row0 = DIRECT ? blockIdx.x / units : a.row0, worker = blockIdx.x;
+    uint32_t peers = 1;
+    if constexpr (DIRECT) asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(peers));
+    const uint32_t worker = DIRECT ? blockIdx.x / peers : blockIdx.x, row0 = DIRECT ? worker / units : a.row0;
     PagedPlace at;
     uint32_t count;
     if constexpr (DIRECT) {
-        if (!paged_direct_enter<HD>(a, list, row0, worker - row0 * units, at)) return;
-        count = at.tiles;
+        if (!paged_direct_enter<HD>(a, list, row0, worker - row0 * units, at)) return;  // the same in every CTA of a cluster
+        if (peers > 1u) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // it is there before anything is stored into it
+        const uint32_t per = (at.tiles + peers - 1u) / peers;
+        at.tile = min(tc::cluster_rank() * per, at.tiles);
+        count = min(per, at.tiles - at.tile);
     } else {
         if (tid < 32u) paged_list_make(a, list, rows, SPAN);
         __syncthreads();
@@ -566,30 +577,71 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                                           own_o + own * HD);
                 }
             }
-            if constexpr (DIRECT) {
-                __syncthreads();
-                for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) {
-                    const uint32_t h = i / HD, d = i % HD;
-                    float m[TILES_WARPS], M = -INFINITY, L = 0.0f, O = 0.0f;
-#pragma unroll
-                    for (uint32_t w = 0; w < TILES_WARPS; ++w) m[w] = warp_part(w)[ROWS * HD + h], M = fmaxf(M, m[w]);
-#pragma unroll
-                    for (uint32_t w = 0; w < TILES_WARPS; ++w) {
-                        const float l = warp_part(w)[ROWS * HD + ROWS + h];
-                        const float e = l != 0.0f ? (m[w] == -INFINITY ? 1.0f : exp2f(m[w] - M)) : 0.0f;  // a sum without a maximum: NaN, as it is
-                        L += l * e;
-                        if (e != 0.0f) O = fmaf(e, warp_part(w)[h * HD + d], O);
-                    }
-                    const size_t head = (size_t)row * a.q_heads + head0 + h;
-                    a.out[head * HD + d] = L == 0.0f ? 0.0f : O / L;
-                    if (a.stat && d == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
-                }
-            }
         }
         entering = paged_list_next(list, at, rows, units, SPAN);
     }
     cp_async_wait<0>();
     if (bad) atomicOr(a.status, 1u);
+    if constexpr (DIRECT) {
+        const uint32_t unit = worker - row0 * units, kvh = unit / subgroups, g0 = (unit - kvh * subgroups) * a.heads_at_once;
+        G = min(a.heads_at_once, a.group - g0);
+        const size_t first_head = (size_t)row0 * a.q_heads + kvh * a.group + g0;
+        if (count == 0 && lane < ROWS) warp_part(warp)[ROWS * HD + lane] = -INFINITY, warp_part(warp)[ROWS * HD + ROWS + lane] = 0.0f;
+        __syncthreads();
+        // n parts with maximum m(i), sum l(i) and output o(i), in their order; a sum without a maximum stays NaN, as it is
+        const auto join = [](uint32_t n, auto m, auto l, auto o, float* M_out, float* L_out) {
+            float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; ++i) M = fmaxf(M, m(i));
+#pragma unroll 4
+            for (uint32_t i = 0; i < n; ++i) {
+                const float e = l(i) != 0.0f ? (m(i) == -INFINITY ? 1.0f : exp2f(m(i) - M)) : 0.0f;
+                L += l(i) * e;
+                if (e != 0.0f) O = fmaf(e, o(i), O);
+            }
+            *M_out = M, *L_out = L;
+            return O;
+        };
+        const auto of_warps = [&](uint32_t i, float* M, float* L) {  // value i of the heads' outputs
+            const uint32_t h = i / HD, d = i % HD;
+            return join(TILES_WARPS, [&](uint32_t w) { return warp_part(w)[ROWS * HD + h]; }, [&](uint32_t w) { return warp_part(w)[ROWS * HD + ROWS + h]; },
+                        [&](uint32_t w) { return warp_part(w)[h * HD + d]; }, M, L);
+        };
+        const auto finish = [&](uint32_t i, float M, float L, float O) {
+            const size_t head = first_head + i / HD;
+            a.out[head * HD + i % HD] = L == 0.0f ? 0.0f : O / L;
+            if (a.stat && i % HD == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+        };
+        float M, L;
+        if (peers == 1u) {
+            for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) {
+                const float O = of_warps(i, &M, &L);
+                finish(i, M, L, O);
+            }
+            return;
+        }
+        const uint32_t me = tc::cluster_rank(), slice = G * HD / peers;  // HD is a multiple of every cluster
+        float* told_m = reinterpret_cast<float*>(smem + Cfg::SMEM);      // [peers][ROWS]
+        float *told_l = told_m + DIRECT_CLUSTER * ROWS, *told_o = told_l + DIRECT_CLUSTER * ROWS;  // [peers][slice]
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        for (uint32_t i = tid; i < G * HD; i += TILES_THREADS) {
+            const float O = of_warps(i, &M, &L);
+            const uint32_t to = i / slice, h = i / HD;
+            tc::st_cluster(tc::map_to_rank(tc::smem_u32(told_o + me * slice + i - to * slice), to), __float_as_uint(O));
+            if (i % HD < peers) {  // one of them tells CTA i % HD
+                tc::st_cluster(tc::map_to_rank(tc::smem_u32(told_m + me * ROWS + h), i % HD), __float_as_uint(M));
+                tc::st_cluster(tc::map_to_rank(tc::smem_u32(told_l + me * ROWS + h), i % HD), __float_as_uint(L));
+            }
+        }
+        __syncwarp();
+        tc::cluster_sync_all();  // the last word between the CTAs: any may leave after it
+        for (uint32_t j = tid; j < slice; j += TILES_THREADS) {
+            const uint32_t i = me * slice + j, h = i / HD;
+            const float O = join(peers, [&](uint32_t c) { return told_m[c * ROWS + h]; }, [&](uint32_t c) { return told_l[c * ROWS + h]; },
+                                 [&](uint32_t c) { return told_o[c * slice + j]; }, &M, &L);
+            finish(i, M, L, O);
+        }
+    }
 }
 
 // The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most 1792, the warps of 444 CTAs);
@@ -783,17 +835,34 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
 bool few_heads(const M40llmCudaContext* ctx, uint32_t q_heads, uint32_t rows) { return (uint64_t)q_heads * rows <= 2ull * (uint64_t)ctx->sm_count; }
 
 template <int HD, bool WIDE, bool DIRECT>
-cudaError_t launch_tiles(M40llmCudaContext* ctx, const PagedAttnArgs& a) {
+cudaError_t launch_tiles(M40llmCudaContext* ctx, const PagedAttnArgs& a, uint32_t peers) {
     using Cfg = TilesCfg<HD, WIDE>;
-    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM);
+    constexpr int smem = Cfg::SMEM + (DIRECT ? Cfg::TOLD : 0);
+    const cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<HD, WIDE, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    return m40_launch_dependent(paged_tiles_kernel<HD, WIDE, DIRECT>, dim3(a.workers), dim3(TILES_THREADS), Cfg::SMEM, ctx->decode_stream, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.workers * peers);
+    cfg.blockDim = dim3(TILES_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->decode_stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = m40_pdl_enabled() ? attr : attr + 1;
+    cfg.numAttrs = m40_pdl_enabled() ? 1 : 0;
+    if (peers > 1u) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = peers;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<HD, WIDE, DIRECT>, a);
 }
 template <bool DIRECT>
-cudaError_t launch_tiles_of(M40llmCudaContext* ctx, const PagedAttnArgs& a) {
+cudaError_t launch_tiles_of(M40llmCudaContext* ctx, const PagedAttnArgs& a, uint32_t peers) {
     const bool wide = a.heads_at_once > 8u;
-    if (a.c.hd == 64u) return wide ? launch_tiles<64, true, DIRECT>(ctx, a) : launch_tiles<64, false, DIRECT>(ctx, a);
-    return wide ? launch_tiles<128, true, DIRECT>(ctx, a) : launch_tiles<128, false, DIRECT>(ctx, a);
+    if (a.c.hd == 64u) return wide ? launch_tiles<64, true, DIRECT>(ctx, a, peers) : launch_tiles<64, false, DIRECT>(ctx, a, peers);
+    return wide ? launch_tiles<128, true, DIRECT>(ctx, a, peers) : launch_tiles<128, false, DIRECT>(ctx, a, peers);
 }
 
 // All rows in launches of up to 256, each followed by its join. `ctas`: how many are resident, `span`: entries of a tile of the list.
@@ -873,9 +942,17 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     }
     const size_t heads = (size_t)c->rows * c->q_heads;
     const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
-    // Short rows: a CTA takes a unit as a whole. One row of 64 entries, 32 / 4 heads of 64: 4.3 us against 6.8, of 500 9.8 against 7.2; 8 rows of up to 500,
-    // 32 / 8 heads of 128: 12.0 against 13.7, 48 rows 24.8 against 28.1, of 1000 alike. (In paged_lanes_kernel it was slower: 9.8 us against 8.5.)
-    const bool direct = tiles && a.bound <= (c->rows * units >= 64u ? 512u : 256u) && c->rows * units <= 0x7fffffffu;
+    // Short rows: clusters of up to 8 CTAs that fill half of the device take a unit each, without a list and a join. How many tiles a CTA may have then: 32
+    // with a wave of CTAs or more, 16 with half of one (the list deals uneven rows better, but its parts and their join cost more the more rows there are), else 4
+    // (the list has more CTAs at work). Us, this against the list: one row of 64 / 700 / 2000 entries, 32 / 4 heads of 64, 4.6 / 6.9 / 8.5 against 6.9 / 7.5 / 8.2;
+    // rows of 32 / 8 heads of 128: 4 of 1000 9.4 (11.0), 8 of up to 500 9.0 (11.8), 8 of 4000 29 (35), 8 of 8000 54.6 (54.7), 32 of 100 to 1000 23.5 (27.3),
+    // 32 of 100 to 2000 38.7 (39.7), 200 of 100 to 500 65 (90), 200 of 100 to 2000 152 (182), 100 of 100 to 4000 160 (159). Clusters of 16 are not placed as they
+    // come free: 2 rows of 1000 14.2 against 8.4 with 8. (paged_lanes_kernel, one CTA a unit: 9.8 against 8.5.)
+    uint32_t peers = 1u;
+    while (peers < DIRECT_CLUSTER && a.bound > SPAN * peers && (uint64_t)c->rows * units * peers * 2u <= ctas) peers *= 2u;
+    const uint64_t direct_ctas = (uint64_t)c->rows * units * peers;
+    const uint32_t most_tiles = direct_ctas >= ctas ? 32u : (2u * direct_ctas >= ctas ? 16u : 4u);
+    const bool direct = tiles && a.bound <= SPAN * peers * most_tiles && direct_ctas <= 0x7fffffffu;
     if ((list && !direct) || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? (a.bound + 3u) & ~3u : 0u;
         const size_t rows_at_once = c->rows < LIST_ROWS ? c->rows : LIST_ROWS;
@@ -896,10 +973,10 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     cudaError_t e;
     if (direct) {
         a.workers = (uint32_t)(c->rows * units);
-        e = launch_tiles_of<true>(ctx, a);
+        e = launch_tiles_of<true>(ctx, a, peers);
         M40_COUNT_LAUNCH(ctx);
     } else if (tiles) {
-        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x); });
+        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x, 1u); });
     } else if (by_lanes) {
         e = launch_list(ctx, a, ctas, 8u * lanes.warps, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
     } else {

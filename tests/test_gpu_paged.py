@@ -193,6 +193,32 @@ def test_attention_large_and_small_scores(nat, kind, dim):
     T.check_attention(c, q, [0, 1], [600, 600], got)
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 32, 4), (128, 16, 2), (128, 16, 1), (64, 9, 1), (128, 3, 3)])
+@pytest.mark.parametrize("rows", [1, 2, 5, 24, 150])
+@pytest.mark.parametrize("entries", [70, 250, 1000, 2000])
+def test_attention_clusters(nat, dim, heads, kv_heads, rows, entries):
+    """Few rows and many, bounds on both sides of the sizes that clusters take; rows shorter than the cluster's shares, empty ones, windows, and their weights."""
+    rng = np.random.default_rng(rows + entries + dim)
+    slots = min(rows, 6)
+    c = T.Cache(nat, rng, slots, entries, kv_heads, dim, 16)
+    slot = np.arange(rows) % slots
+    length = rng.integers(0, entries + 1, rows)
+    length[0] = entries
+    if rows > 3:
+        length[1:4] = 0, 1, 65
+    begin = np.where(rng.random(rows) < 0.3, length // 2, 0)
+    q = (2 * rng.standard_normal((rows, heads, dim))).astype(np.float32)
+    some = np.unique(np.r_[0, rng.integers(0, rows, 6), np.minimum(rows - 1, [1, 2, 3])])
+    got, _ = T.attend(nat, c, q, slot, length, begin=begin, max_len=entries)
+    T.check_attention(c, q[some], slot[some], length[some], got[some], begin=begin[some])
+    again, _ = T.attend(nat, c, q, slot, length, begin=begin, max_len=entries)
+    assert np.array_equal(got, again) and T.status(nat) == 0
+    if rows <= 5:
+        w = rng.random((slots, kv_heads, c.capacity)).astype(np.float32)
+        got, gw = T.attend(nat, c, q, slot, length, begin=begin, max_len=entries, weights=w, ld=c.capacity, in_place=True)
+        T.check_attention(c, q, slot, length, got, begin=begin, weights=w, got_w=gw, before=w)
+
+
 @pytest.mark.parametrize("kind,dim,heads", [("f16", 128, 8), ("f16", 64, 12), ("f32", 64, 8), ("f16", 40, 8)])
 @pytest.mark.parametrize("queries,keys", [(1e-5, 4096.0), (1e-12, 8192.0), (1e6, 1e-3)])
 def test_attention_sizes_of_queries_and_keys(nat, kind, dim, heads, queries, keys):
