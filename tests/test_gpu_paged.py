@@ -147,11 +147,11 @@ def test_attention_window(nat, kind, dim, heads):
 
 
 @pytest.mark.parametrize("kind,dim,offset", [("f16", 128, 0), ("f16", 64, 0), ("f16", 64, 1), ("f32", 64, 0), ("f32", 64, 1), ("f16", 36, 0), ("f16", 96, 0)])
-@pytest.mark.parametrize("max_len", [0, 200])
-def test_attention_ignores_what_is_masked(nat, kind, dim, offset, max_len):
+@pytest.mark.parametrize("entries,max_len", [(300, 0), (300, 200), (5000, 0)])
+def test_attention_ignores_what_is_masked(nat, kind, dim, offset, entries, max_len):
     """Infinities and NaN behind a row's entries, before its window, on its last page and on other pages do not reach the output."""
     rng = np.random.default_rng(dim + offset)
-    c = T.Cache(nat, rng, 4, 300, 2, dim, 16, kind, offset=offset)
+    c = T.Cache(nat, rng, 4, entries, 2, dim, 16, kind, offset=offset)
     length, begin = [1, 130, 200, 64], [0, 3, 70, 0]
     q = (2 * rng.standard_normal((4, 8, dim))).astype(np.float32)
     seen = np.zeros((c.pages, 16), bool)
@@ -167,7 +167,7 @@ def test_attention_ignores_what_is_masked(nat, kind, dim, offset, max_len):
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 128), ("f32", 128)])
-@pytest.mark.parametrize("n", [300, 230])
+@pytest.mark.parametrize("n", [300, 230, 5000])
 def test_attention_values_that_are_not_finite(nat, kind, dim, n):
     """What a row does see reaches its output as the formula says; the rows beside it keep theirs."""
     rng = np.random.default_rng(1)
@@ -219,12 +219,42 @@ def test_attention_clusters(nat, dim, heads, kv_heads, rows, entries):
         T.check_attention(c, q, slot, length, got, begin=begin, weights=w, got_w=gw, before=w)
 
 
+@pytest.mark.parametrize("kind,dim,heads,kv_heads,page", [("f16", 64, 32, 4, 16), ("f16", 128, 16, 2, 1), ("f16", 128, 40, 2, 128), ("f16", 64, 17, 1, 2),
+                                                          ("f16", 128, 4, 4, 64), ("f32", 128, 8, 1, 16), ("f16", 96, 6, 2, 4), ("f16", 33, 4, 2, 16)])
+@pytest.mark.parametrize("rows", [9, 270])
+def test_attention_long_bounds(nat, kind, dim, heads, kv_heads, page, rows):
+    """A bound of 20000 entries for rows of any length: the smallest, empty ones, windows, a page outside the pool, rows outside the cache, and weights."""
+    rng = np.random.default_rng(rows + page + dim)
+    c = T.Cache(nat, rng, 9, 20000, kv_heads, dim, page, kind)
+    slot = np.arange(rows) % 9
+    length = rng.choice(LENS, rows)
+    length[:9] = 3000, 1, 0, 77, 64, 5000, 16, 2, 400
+    begin = np.where(rng.random(rows) < 0.3, length // 2, 0)
+    begin[:9] = 0, 0, 0, 5, 64, 1003, 0, 0, 0
+    c.table[8, 130 // page] = c.pages  # entry 130 of slot 8
+    c.upload()
+    q = (2 * rng.standard_normal((rows, heads, dim))).astype(np.float32)
+    some = np.unique(np.r_[np.arange(9), rng.integers(0, rows, 20)])
+    got, _ = T.attend(nat, c, q, slot, length, begin=begin)
+    T.check_attention(c, q[some], slot[some], length[some], got[some], begin=begin[some])
+    assert T.status(nat) == 1 and not got[length <= begin].any()
+    w = rng.random((9, kv_heads, c.capacity)).astype(np.float32)
+    got, gw = T.attend(nat, c, q[:9], slot[:9], length[:9], begin=begin[:9], weights=w, ld=c.capacity, in_place=True)
+    T.check_attention(c, q[:9], slot[:9], length[:9], got, begin=begin[:9], weights=w, got_w=gw, before=w)
+    outside = length.copy()
+    outside[3], slot[4] = c.capacity + 1, 9
+    got2, _ = T.attend(nat, c, q, slot, outside, begin=begin)
+    assert not got2[3:5].any() and np.array_equal(got2[5:9], T.attend(nat, c, q, slot, outside, begin=begin)[0][5:9]) and T.status(nat) == 1
+    T.check_attention(c, q[5:9], slot[5:9], length[5:9], got2[5:9], begin=begin[5:9])
+
+
 @pytest.mark.parametrize("kind,dim,heads", [("f16", 128, 8), ("f16", 64, 12), ("f32", 64, 8), ("f16", 40, 8)])
 @pytest.mark.parametrize("queries,keys", [(1e-5, 4096.0), (1e-12, 8192.0), (1e6, 1e-3)])
-def test_attention_sizes_of_queries_and_keys(nat, kind, dim, heads, queries, keys):
+@pytest.mark.parametrize("entries", [600, 5000])
+def test_attention_sizes_of_queries_and_keys(nat, kind, dim, heads, queries, keys, entries):
     """Queries far from 1 keep their bits: the scores are what they are for queries and keys that share the size."""
     rng = np.random.default_rng(3)
-    c = T.Cache(nat, rng, 2, 600, 1, dim, 16, kind)
+    c = T.Cache(nat, rng, 2, entries, 1, dim, 16, kind)
     c.k = (c.k.astype(np.float32) * np.float32(keys)).astype(c.dtype)
     c.upload()
     q = (queries * rng.standard_normal((2, heads, dim))).astype(np.float32)
@@ -233,7 +263,7 @@ def test_attention_sizes_of_queries_and_keys(nat, kind, dim, heads, queries, key
 
 
 @pytest.mark.parametrize("kind,dim", [("f16", 128), ("f32", 64), ("f16", 20)])
-@pytest.mark.parametrize("n", [100, 700])
+@pytest.mark.parametrize("n", [100, 700, 5000])
 def test_attention_weights_where_nothing_is_seen(nat, kind, dim, n):
     """Rows whose pages are all outside the pool, and rows whose scores are all -inf: zeros, and the weights stay."""
     rng = np.random.default_rng(4)
@@ -351,10 +381,11 @@ def test_attention_beyond_32_bits(nat, dim):
     assert T.status(nat) == 0
 
 
-def test_attention_captured(nat):
+@pytest.mark.parametrize("entries", [2000, 9000])
+def test_attention_captured(nat, entries):
     """A captured step is replayed while lengths and tables change; a second graph, captured later and larger, leaves the first one right."""
     rng = np.random.default_rng(9)
-    c = T.Cache(nat, rng, 3, 2000, 2, 128, 16)
+    c = T.Cache(nat, rng, 3, entries, 2, 128, 16)
     q = rng.standard_normal((3, 8, 128)).astype(np.float32)
     w = np.zeros((3, 2, c.capacity), np.float32)
     L = nat.lib
