@@ -648,12 +648,12 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
 // then 256 / LANES groups of lanes take every so-many-th part, each lane V dimensions, and the groups' sums meet in shared memory. CTAs of 8 lanes share a
 // head's dimensions where there are few heads, for more loads at a time.
 template <int V, int LANES, typename Part>
-__device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t parts, Part part) {
+__device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t share, uint32_t parts, Part part) {
     constexpr uint32_t MOST = 1792, GROUPS = 256 / LANES, AT_ONCE = 4;
     __shared__ float sw[MOST], red[16];
     __shared__ float s_acc[8][LANES * V];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
-    const uint32_t vl = tid % LANES, group = tid / LANES, d = (blockIdx.z * LANES + vl) * V;
+    const uint32_t vl = tid % LANES, group = tid / LANES, d = (share * LANES + vl) * V;
     float x[AT_ONCE][V];
     const auto fetch = [&](uint32_t s0) {
 #pragma unroll
@@ -698,7 +698,7 @@ __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t 
     L = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) L += red[8 + i];
-    if (a.stat && tid == 0 && blockIdx.z == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
+    if (a.stat && tid == 0 && share == 0) a.stat[2 * head] = M == -INFINITY ? 0.0f : M, a.stat[2 * head + 1] = L == 0.0f ? 0.0f : 1.0f / L;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
@@ -723,7 +723,7 @@ __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t 
         for (int i = 0; i < V; ++i) s_acc[warp][i * LANES + lane] = acc[i];
     __syncthreads();
     if (tid < LANES * V) {  // value tid: i = tid / LANES of lane tid % LANES
-        const uint32_t at = (blockIdx.z * LANES + tid % LANES) * V + tid / LANES;
+        const uint32_t at = (share * LANES + tid % LANES) * V + tid / LANES;
         float o = 0.0f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) o += s_acc[w][tid];
@@ -737,39 +737,83 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
     pdl_wait();
     pdl_trigger();
     const size_t head = (size_t)blockIdx.y * a.q_heads + blockIdx.x, base = head * a.splits;
-    paged_join_parts<V, LANES>(a, head, a.splits, [=](uint32_t s) { return base + s; });
+    paged_join_parts<V, LANES>(a, head, blockIdx.z, a.splits, [=](uint32_t s) { return base + s; });
 }
 
-// Parts of paged_tiles_kernel and paged_lanes_kernel, and the zeros of rows without entries. Grid (q head, row of the launch, share of the dimensions).
+// Of one q head of row r of a launch of `rows`: how many parts the warps left, and where. Nothing for a row without entries.
+struct PagedParts {
+    uint32_t n, first, h;
+    __device__ __forceinline__ size_t at(const PagedAttnArgs& a, uint32_t s) const { return ((size_t)first + s) * a.heads_at_once + h; }
+};
+struct PagedBefore {  // tiles before the row, before the next one, of all rows
+    uint64_t row, next, all;
+};
+__device__ __forceinline__ PagedBefore paged_before(const PagedAttnArgs& a, uint32_t r, uint32_t rows) {
+    return PagedBefore{a.prefix[r], a.prefix[r + 1], a.prefix[rows]};
+}
+__device__ __forceinline__ PagedParts paged_parts(const PagedAttnArgs& a, uint32_t r, const PagedBefore& b, uint32_t q_head) {
+    const uint32_t kvh = q_head / a.group, in_group = q_head - kvh * a.group;
+    const uint32_t subgroups = (a.group + a.heads_at_once - 1u) / a.heads_at_once, units = a.c.kv_heads * subgroups;
+    const uint32_t unit = kvh * subgroups + in_group / a.heads_at_once;
+    const uint64_t before = b.row, tiles = b.next - before, total = b.all * units;
+    if (tiles == 0) return PagedParts{0u, 0u, 0u};
+    const uint32_t n = ctas_at_work(total, a.workers);
+    const uint64_t lo = before * units + unit * tiles;
+    const uint32_t w0 = cta_of(lo, total, n), w1 = cta_of(lo + tiles - 1u, total, n);
+    return PagedParts{(w1 - w0 + 1u) * a.part_warps, (r * units + unit + w0) * a.part_warps, in_group % a.heads_at_once};
+}
+
+// Parts of paged_tiles_kernel and paged_lanes_kernel, and the zeros of rows without entries: a q head of row r, a share of the dimensions.
+template <int LANES>
+__device__ __forceinline__ void paged_join_head(const PagedAttnArgs& a, uint32_t r, uint32_t rows, uint32_t q_head, uint32_t share) {
+    const size_t head = (size_t)(a.row0 + r) * a.q_heads + q_head;
+    const PagedParts parts = paged_parts(a, r, paged_before(a, r, rows), q_head);
+    if (parts.n == 0) {
+        if (share == 0)
+            for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
+        return;
+    }
+    paged_join_parts<4, LANES>(a, head, share, parts.n, [&](uint32_t s) { return parts.at(a, s); });
+}
+// Grid (q head, row of the launch, share of the dimensions).
 template <int LANES>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedAttnArgs a) {
     pdl_wait();
     pdl_trigger();
-    const uint32_t r = blockIdx.y, rows = gridDim.y, kvh = blockIdx.x / a.group, in_group = blockIdx.x - kvh * a.group;
-    const uint32_t subgroups = (a.group + a.heads_at_once - 1u) / a.heads_at_once, units = a.c.kv_heads * subgroups;
-    const uint32_t unit = kvh * subgroups + in_group / a.heads_at_once, h = in_group % a.heads_at_once;
-    const size_t head = (size_t)(a.row0 + r) * a.q_heads + blockIdx.x;
-    const uint64_t before = a.prefix[r], tiles = a.prefix[r + 1] - before, total = a.prefix[rows] * units;
-    if (tiles == 0) {
-        if (blockIdx.z == 0)
-            for (uint32_t d = threadIdx.x; d < a.c.hd; d += 256u) a.out[head * a.c.hd + d] = 0.0f;
-        return;
+    paged_join_head<LANES>(a, blockIdx.y, gridDim.y, blockIdx.x, blockIdx.z);
+}
+
+// A head's maximum and 1 / sum from its parts, by a warp: what paged_join_parts leaves in a.stat.
+__device__ __forceinline__ float2 paged_parts_stat(const PagedAttnArgs& a, const PagedParts& parts) {
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+    for (uint32_t s = threadIdx.x & 31u; s < parts.n; s += 32u) {
+        const float l = a.part_l[parts.at(a, s)], m = a.part_m[parts.at(a, s)];
+        const float top = fmaxf(M, m), use = top == -INFINITY ? 0.0f : top;  // a sum without a maximum: NaN, as it is
+        L = (M == -INFINITY ? L : L * exp2f(M - use)) + (l == 0.0f ? 0.0f : (m == -INFINITY ? l : l * exp2f(m - use)));
+        M = top;
     }
-    const uint32_t n = ctas_at_work(total, a.workers);
-    const uint64_t lo = before * units + unit * tiles;
-    const uint32_t w0 = cta_of(lo, total, n), w1 = cta_of(lo + tiles - 1u, total, n);
-    const size_t part = ((size_t)r * units + unit + w0) * a.part_warps;
-    paged_join_parts<4, LANES>(a, head, (w1 - w0 + 1u) * a.part_warps, [=](uint32_t s) { return (part + s) * a.heads_at_once + h; });
+    const float top = warp_max(M);
+    L = warp_sum(M == -INFINITY ? L : L * exp2f(M - top));
+    return make_float2(top == -INFINITY ? 0.0f : top, L == 0.0f ? 0.0f : 1.0f / L);
 }
 
 // CTA = (1024 entries, kv head, row); only the first row of a slot works, for all rows of the slot in their order, so that sums do not
 // depend on who comes first. Thread = four neighbouring entries (one after the other where weights or scores are not 16-byte aligned).
-// Bound by the scores, which mostly come out of L2.
-constexpr uint32_t WEIGHTS_AT_ONCE = 1024;
-__global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uint32_t vec) {
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, row = blockIdx.z, h = blockIdx.y;
+// PARTS: the statistics come from the parts, not from a.stat. Bound by the chain rows, parts and scores, weights.
+constexpr uint32_t WEIGHTS_AT_ONCE = 1024, WEIGHTS_GROUP = 64, WEIGHTS_HEADS = 4;
+template <bool PARTS>
+__device__ __forceinline__ void paged_weights(const PagedAttnArgs& a, uint32_t vec, uint32_t piece, uint32_t h, uint32_t row) {
+    __shared__ float2 s_stat[PARTS ? WEIGHTS_GROUP : 1];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, e0 = piece * WEIGHTS_AT_ONCE, e = e0 + 4u * tid;
+    float4 x[WEIGHTS_HEADS];  // scores of up to four heads
+    const auto fetch = [&](size_t head, uint32_t g0, uint32_t to) {
+#pragma unroll
+        for (uint32_t g = 0; g < WEIGHTS_HEADS; ++g)
+            if (g0 + g < a.group && e < to) x[g] = *reinterpret_cast<const float4*>(a.scores + (head + g0 + g) * a.ld_scores + e);
+    };
+    PagedBefore tiles_before{};
+    if (PARTS) tiles_before = paged_before(a, row, a.rows);
     const uint32_t slot = a.row_slot[row];
     if (slot >= a.c.slots) return;
     // every warp looks at all rows, 32 at a time, a lane each
@@ -782,14 +826,13 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
     }
     if (__any_sync(0xffffffffu, skip)) return;
     most = __reduce_max_sync(0xffffffffu, most);
-    const uint32_t e = blockIdx.x * WEIGHTS_AT_ONCE + 4u * tid;
-    if (blockIdx.x * WEIGHTS_AT_ONCE >= most) return;
+    if (e0 >= most) return;
     const size_t at = ((size_t)slot * a.c.kv_heads + h) * a.ld_weights + e;
     const bool whole = vec && e + 4u <= most;
     float w[4];
     if (whole && a.weights_in) {
-        const float4 x = *reinterpret_cast<const float4*>(a.weights_in + at);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        const float4 y = *reinterpret_cast<const float4*>(a.weights_in + at);
+        w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) w[i] = a.weights_in && e + i < most ? a.weights_in[at + i] : 0.0f;
@@ -798,24 +841,33 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
         const uint32_t r = r0 + lane;
         if (a.rows > 32u && r < a.rows) paged_row_range(a, r, &s, &b, &n);  // up to 32 are there already
         uint32_t mask = __ballot_sync(0xffffffffu, r < a.rows && s == slot);
-        while (mask) {  // the slot's rows in order
-            const uint32_t k = __ffs(mask) - 1u, from = __shfl_sync(0xffffffffu, b, k), to = __shfl_sync(0xffffffffu, n, k);
+        while (mask) {  // the slot's rows in order, `row` the first
+            const uint32_t k = __ffs(mask) - 1u, from = __shfl_sync(0xffffffffu, b, k), to = __shfl_sync(0xffffffffu, n, k), now = r0 + k;
             mask &= mask - 1u;
+            if (from >= to || e0 >= to || e0 + WEIGHTS_AT_ONCE <= from) continue;  // the same for all threads
+            const size_t head = (size_t)now * a.q_heads + h * a.group;
+            fetch(head, 0u, to);  // on their way while the statistics are made
+            if constexpr (PARTS) {
+                __syncthreads();
+                const PagedBefore before = now == row ? tiles_before : paged_before(a, now, a.rows);
+                for (uint32_t g = tid >> 5; g < a.group; g += 8u) {
+                    const float2 y = paged_parts_stat(a, paged_parts(a, now, before, h * a.group + g));
+                    if (lane == 0) s_stat[g] = y;
+                }
+                __syncthreads();
+            }
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            const size_t head = (size_t)(r0 + k) * a.q_heads + h * a.group;
-            const bool all = whole && e >= from && e + 4u <= to;
-#pragma unroll 4
-            for (uint32_t g = 0; g < a.group; ++g) {
-                const float M = a.stat[2 * (head + g)], inv = a.stat[2 * (head + g) + 1];
-                const float* sc = a.scores + (head + g) * a.ld_scores + e;
-                if (all) {
-                    const float4 x = *reinterpret_cast<const float4*>(sc);
-                    sum[0] += exp2f(x.x - M) * inv, sum[1] += exp2f(x.y - M) * inv;
-                    sum[2] += exp2f(x.z - M) * inv, sum[3] += exp2f(x.w - M) * inv;
-                } else {
+            for (uint32_t g0 = 0; g0 < a.group; g0 += WEIGHTS_HEADS) {
+                if (g0) fetch(head, g0, to);
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i)
-                        if (e + i >= from && e + i < to) sum[i] += exp2f(sc[i] - M) * inv;
+                for (uint32_t j = 0; j < WEIGHTS_HEADS; ++j) {
+                    const uint32_t g = g0 + j;
+                    if (g >= a.group) break;
+                    const float M = PARTS ? s_stat[g].x : a.stat[2 * (head + g)], inv = PARTS ? s_stat[g].y : a.stat[2 * (head + g) + 1];
+                    sum[0] += e >= from && e < to ? exp2f(x[j].x - M) * inv : 0.0f;
+                    sum[1] += e + 1u >= from && e + 1u < to ? exp2f(x[j].y - M) * inv : 0.0f;
+                    sum[2] += e + 2u >= from && e + 2u < to ? exp2f(x[j].z - M) * inv : 0.0f;
+                    sum[3] += e + 3u >= from && e + 3u < to ? exp2f(x[j].w - M) * inv : 0.0f;
                 }
             }
 #pragma unroll
@@ -828,6 +880,27 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uin
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i)
             if (e + i < most) a.weights_out[at + i] = w[i];
+    }
+}
+__global__ void __launch_bounds__(256) paged_weights_kernel(PagedAttnArgs a, uint32_t vec) {
+    pdl_wait();
+    pdl_trigger();
+    paged_weights<false>(a, vec, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+// Weights and join side by side: `weighing` CTAs of paged_weights (piece of the entries, kv head, row), which look at the parts themselves instead of waiting for
+// the join, then those of the join (q head, row, share). All rows are in one launch. Us of the whole call against one after the other: 12 rows of 509 to
+// 8192 entries, 32 / 8 heads of 128, 53.4 (55.9), one of 8192 18.6 (19.9), 60 of 500 to 3000 103 (103), 9 of f32 24.5 (27.8). 64 registers, and the parts one by one: with
+// four of them at a time 56.3, with 85 registers 53.5 and 106, with 51 55.4 and 106.
+template <int LANES>
+__global__ void __launch_bounds__(256, 4) paged_join_weights_kernel(PagedAttnArgs a, uint32_t vec, uint32_t weighing, uint32_t pieces) {
+    pdl_wait();
+    pdl_trigger();
+    if (blockIdx.x < weighing) {
+        const uint32_t x = blockIdx.x / pieces, row = x / a.c.kv_heads;
+        paged_weights<true>(a, vec, blockIdx.x - x * pieces, x - row * a.c.kv_heads, row);
+    } else {
+        const uint32_t b = blockIdx.x - weighing, x = b / a.q_heads, share = x / a.rows;
+        paged_join_head<LANES>(a, x - share * a.rows, a.rows, b - x * a.q_heads, share);
     }
 }
 
@@ -867,10 +940,24 @@ cudaError_t launch_tiles_of(M40llmCudaContext* ctx, const PagedAttnArgs& a, uint
 
 // All rows in launches of up to 256, each followed by its join. `ctas`: how many are resident, `span`: entries of a tile of the list.
 template <typename Launch>
-cudaError_t launch_list(M40llmCudaContext* ctx, PagedAttnArgs a, uint32_t ctas, uint32_t span, Launch launch) {
+cudaError_t launch_list(M40llmCudaContext* ctx, PagedAttnArgs a, uint32_t ctas, uint32_t span, uint32_t vec, bool* weighed, Launch launch) {
     const uint64_t most = (uint64_t)a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once) * ((a.bound + span - 1u) / span) * a.rows;
     a.workers = most < ctas ? (uint32_t)most : ctas;
     cudaError_t e = cudaSuccess;
+    const bool few = few_heads(ctx, a.q_heads, a.rows);
+    const uint32_t pieces = (a.bound + WEIGHTS_AT_ONCE - 1u) / WEIGHTS_AT_ONCE;
+    const uint64_t joins = (uint64_t)a.q_heads * a.rows * (few ? (a.c.hd + 31u) / 32u : (a.c.hd + 127u) / 128u);
+    const uint64_t weighing = (uint64_t)pieces * a.c.kv_heads * a.rows, both = joins + weighing;
+    *weighed = a.scores && a.rows <= LIST_ROWS && a.group <= WEIGHTS_GROUP && both <= 0x7fffffffu;
+    if (*weighed) {
+        e = launch(a);
+        if (e == cudaSuccess)
+            e = m40_launch_dependent(few ? paged_join_weights_kernel<8> : paged_join_weights_kernel<32>, dim3((uint32_t)both), dim3(256), 0, ctx->decode_stream, a, vec,
+                                     (uint32_t)weighing, pieces);
+        M40_COUNT_LAUNCH(ctx);
+        M40_COUNT_LAUNCH(ctx);
+        return e;
+    }
     for (a.row0 = 0; e == cudaSuccess && a.row0 < a.rows; a.row0 += LIST_ROWS) {
         const uint32_t rows = a.rows - a.row0 < LIST_ROWS ? a.rows - a.row0 : LIST_ROWS, hd = a.c.hd;
         e = launch(a);
@@ -970,15 +1057,18 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
             a.scores = a.part_o + ((parts * (hd + 2) + heads * 2 + 3) & ~(size_t)3);  // 16-byte aligned
         }
     }
+    const bool aligned = ((((uintptr_t)a.weights_in) | ((uintptr_t)a.weights_out) | ((uintptr_t)a.scores)) & 15u) == 0 && a.ld_weights % 4u == 0;
+    const uint32_t vec_weights = aligned ? 1u : 0u;
+    bool weighed = false;
     cudaError_t e;
     if (direct) {
         a.workers = (uint32_t)(c->rows * units);
         e = launch_tiles_of<true>(ctx, a, peers);
         M40_COUNT_LAUNCH(ctx);
     } else if (tiles) {
-        e = launch_list(ctx, a, ctas, SPAN, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x, 1u); });
+        e = launch_list(ctx, a, ctas, SPAN, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x, 1u); });
     } else if (by_lanes) {
-        e = launch_list(ctx, a, ctas, 8u * lanes.warps, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
+        e = launch_list(ctx, a, ctas, 8u * lanes.warps, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
     } else {
         const uint32_t elem = f32 ? 4u : 2u, hd4 = (hd + 3u) & ~3u;
         const uint32_t T = hd4 * elem > 1024u ? 16u : 32u, pitch = ((hd4 * elem + 15u) & ~15u) / elem + 16u / elem;
@@ -1007,10 +1097,9 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
             M40_COUNT_LAUNCH(ctx);
         }
     }
-    if (e == cudaSuccess && a.scores) {
-        const bool aligned = ((((uintptr_t)a.weights_in) | ((uintptr_t)a.weights_out) | ((uintptr_t)a.scores)) & 15u) == 0 && a.ld_weights % 4u == 0;
+    if (e == cudaSuccess && a.scores && !weighed) {
         e = m40_launch_dependent(paged_weights_kernel, dim3((a.bound + WEIGHTS_AT_ONCE - 1u) / WEIGHTS_AT_ONCE, cache->kv_heads, c->rows), dim3(256), 0, s, a,
-                                 aligned ? 1u : 0u);
+                                 vec_weights);
         M40_COUNT_LAUNCH(ctx);
     }
     if (e != cudaSuccess) {
