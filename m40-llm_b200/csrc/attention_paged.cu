@@ -9,6 +9,7 @@
 #include "attention_paged.cuh"
 #include "stack_math.cuh"
 #include "tc_ptx.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -588,23 +589,28 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         const size_t first_head = (size_t)row0 * a.q_heads + kvh * a.group + g0;
         if (count == 0 && lane < ROWS) warp_part(warp)[ROWS * HD + lane] = -INFINITY, warp_part(warp)[ROWS * HD + ROWS + lane] = 0.0f;
         __syncthreads();
-        // n parts with maximum m(i), sum l(i) and output o(i), in their order; a sum without a maximum stays NaN, as it is
-        const auto join = [](uint32_t n, auto m, auto l, auto o, float* M_out, float* L_out) {
-            float M = -INFINITY, L = 0.0f, O = 0.0f;
-#pragma unroll 4
-            for (uint32_t i = 0; i < n; ++i) M = fmaxf(M, m(i));
-#pragma unroll 4
-            for (uint32_t i = 0; i < n; ++i) {
-                const float e = l(i) != 0.0f ? (m(i) == -INFINITY ? 1.0f : exp2f(m(i) - M)) : 0.0f;
-                L += l(i) * e;
-                if (e != 0.0f) O = fmaf(e, o(i), O);
+        // up to 8 parts with maximum m(i), sum l(i) and output o(i), in their order, all on their way first; a sum without a maximum stays NaN, as it is
+        const auto join = [](auto most, uint32_t n, auto m, auto l, auto o, float* M_out, float* L_out) {
+            constexpr uint32_t N = decltype(most)::value;
+            float pm[N], pl[N], po[N], M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const bool in = i < n;
+                pm[i] = in ? m(i) : -INFINITY, pl[i] = in ? l(i) : 0.0f, po[i] = in ? o(i) : 0.0f;
+                M = fmaxf(M, pm[i]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const float e = pl[i] != 0.0f ? (pm[i] == -INFINITY ? 1.0f : exp2f(pm[i] - M)) : 0.0f;
+                L += pl[i] * e;
+                if (e != 0.0f) O = fmaf(e, po[i], O);
             }
             *M_out = M, *L_out = L;
             return O;
         };
         const auto of_warps = [&](uint32_t i, float* M, float* L) {  // value i of the heads' outputs
             const uint32_t h = i / HD, d = i % HD;
-            return join(TILES_WARPS, [&](uint32_t w) { return warp_part(w)[ROWS * HD + h]; }, [&](uint32_t w) { return warp_part(w)[ROWS * HD + ROWS + h]; },
+            return join(std::integral_constant<uint32_t, TILES_WARPS>(), TILES_WARPS, [&](uint32_t w) { return warp_part(w)[ROWS * HD + h]; }, [&](uint32_t w) { return warp_part(w)[ROWS * HD + ROWS + h]; },
                         [&](uint32_t w) { return warp_part(w)[h * HD + d]; }, M, L);
         };
         const auto finish = [&](uint32_t i, float M, float L, float O) {
@@ -637,7 +643,7 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
         tc::cluster_sync_all();  // the last word between the CTAs: any may leave after it
         for (uint32_t j = tid; j < slice; j += TILES_THREADS) {
             const uint32_t i = me * slice + j, h = i / HD;
-            const float O = join(peers, [&](uint32_t c) { return told_m[c * ROWS + h]; }, [&](uint32_t c) { return told_l[c * ROWS + h]; },
+            const float O = join(std::integral_constant<uint32_t, DIRECT_CLUSTER>(), peers, [&](uint32_t c) { return told_m[c * ROWS + h]; }, [&](uint32_t c) { return told_l[c * ROWS + h]; },
                                  [&](uint32_t c) { return told_o[c * slice + j]; }, &M, &L);
             finish(i, M, L, O);
         }
@@ -1031,10 +1037,11 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
     // Short rows: clusters of up to 8 CTAs that fill half of the device take a unit each, without a list and a join. How many tiles a CTA may have then: 32
     // with a wave of CTAs or more, 16 with half of one (the list deals uneven rows better, but its parts and their join cost more the more rows there are), else 4
-    // (the list has more CTAs at work). Us, this against the list: one row of 64 / 700 / 2000 entries, 32 / 4 heads of 64, 4.6 / 6.9 / 8.5 against 6.9 / 7.5 / 8.2;
-    // rows of 32 / 8 heads of 128: 4 of 1000 9.4 (11.0), 8 of up to 500 9.0 (11.8), 8 of 4000 29 (35), 8 of 8000 54.6 (54.7), 32 of 100 to 1000 23.5 (27.3),
+    // (the list has more CTAs at work). Us, this against the list: one row of 64 / 700 / 2000 entries, 32 / 4 heads of 64, 4.9 / 6.7 / 8.3 against 6.9 / 7.5 / 8.2;
+    // rows of 32 / 8 heads of 128: 4 of 1000 9.3 (11.0), 8 of up to 500 9.0 (11.8), 8 of 4000 29 (35), 8 of 8000 54.6 (54.7), 32 of 100 to 1000 23.5 (27.3),
     // 32 of 100 to 2000 38.7 (39.7), 200 of 100 to 500 65 (90), 200 of 100 to 2000 152 (182), 100 of 100 to 4000 160 (159). Clusters of 16 are not placed as they
-    // come free: 2 rows of 1000 14.2 against 8.4 with 8. (paged_lanes_kernel, one CTA a unit: 9.8 against 8.5.)
+    // come free: 2 rows of 1000 14.2 against 8.4 with 8. (In paged_lanes_kernel the list is
+    // as fast or faster: 4 rows of up to 250 f32 entries 8.6 and 8.6, one of 700 11.1 against 8.2.)
     uint32_t peers = 1u;
     while (peers < DIRECT_CLUSTER && a.bound > SPAN * peers && (uint64_t)c->rows * units * peers * 2u <= ctas) peers *= 2u;
     const uint64_t direct_ctas = (uint64_t)c->rows * units * peers;

@@ -8,6 +8,8 @@ namespace {
 using namespace attn_mma;
 
 constexpr uint32_t LANES_TILE = 8, LANES_STAGES = 3;  // entries of a warp's tile
+// Where the warps' rings begin: behind their weights (doubled) and corrections, on 16 bytes, as copies want it.
+__host__ __device__ constexpr uint32_t lanes_rings(uint32_t warps, uint32_t gt) { return (warps * (LANES_TILE * gt * 8u + gt * 4u) + 15u) & ~15u; }
 
 __device__ __forceinline__ uint64_t pair_of(float x, float y) {
     uint64_t r;
@@ -49,7 +51,7 @@ __device__ __forceinline__ float xor_sum(float keep, float send, int mask) { ret
 //   softmax  online in base 2, over the lanes with the same head.
 //   outputs  lane = four neighbouring dimensions (DV times); weights come from shared memory, doubled, for two multiply-adds an instruction.
 // hd <= 64 DQ = 128 DV. Bound by HBM. Against 32-entry tiles for the CTA with four barriers each (paged_rows_kernel): 9 rows of up to 4097 f32 entries
-// 46.5 -> 21.3 us.
+// 46.5 -> 20.0 us.
 template <typename ET, int GT, int DQ>
 __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
     constexpr int DV = DQ / 2, HPL = GT == 8 ? 2 : 1;
@@ -60,7 +62,7 @@ __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
     // the warp's memory: weights [8][GT] doubled, corrections [GT], then the ring: K and V of a stage after each other
     float2* s_p = reinterpret_cast<float2*>(smem) + warp * (LANES_TILE * GT);
     float* s_corr = reinterpret_cast<float*>(smem + warps * (LANES_TILE * GT * 8u)) + warp * GT;
-    unsigned char* ring = smem + warps * (LANES_TILE * GT * 8u + GT * 4u) + warp * (LANES_STAGES * 2u * tile_bytes);
+    unsigned char* ring = smem + lanes_rings(warps, GT) + warp * (LANES_STAGES * 2u * tile_bytes);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     const uint32_t units = a.c.kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once), subgroups = units / a.c.kv_heads;
     const uint32_t rows = min(a.rows - a.row0, LIST_ROWS);
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(256, 1) paged_lanes_kernel(PagedAttnArgs a) {
 }
 
 uint32_t lanes_smem(uint32_t warps, uint32_t gt, uint32_t rb) {
-    return warps * (LANES_TILE * gt * 8u + gt * 4u + LANES_STAGES * 2u * LANES_TILE * rb);
+    return lanes_rings(warps, gt) + warps * (LANES_STAGES * 2u * LANES_TILE * rb);
 }
 uint32_t lanes_gt(uint32_t heads) { return heads > 4u ? 8u : (heads > 2u ? 4u : 2u); }
 
@@ -302,8 +304,10 @@ bool m40_paged_lanes(const M40llmCudaContext* ctx, const M40llmPagedCache* cache
     // what the registers hold of queries and outputs: 8 heads of 128 dimensions
     const uint32_t most = cache->head_dim <= 128u ? 8u : (cache->head_dim <= 256u ? 4u : 2u), shares = (group + most - 1u) / most;
     out->heads_at_once = (group + shares - 1u) / shares;
-    out->warps = rb <= 512u ? 8u : (rb <= 1024u ? 4u : 2u);
-    out->ctas = (uint32_t)ctx->sm_count;
+    // Rings of up to 100 KB and two CTAs on an SM, so that the next launch's CTAs find room as these end: 9 rows of up to 4097 f32 entries 20.0 us, with one CTA of
+    // twice the warps 20.9, one row of 64 entries 7.7 against 9.0.
+    out->warps = rb <= 512u ? 4u : (rb <= 1024u ? 2u : 1u);
+    out->ctas = 2u * (uint32_t)ctx->sm_count;
     return true;
 }
 
