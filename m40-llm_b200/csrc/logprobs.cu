@@ -456,7 +456,7 @@ extern "C" int m40llm_logprobs_f32_async(M40llmCudaContext* ctx, const M40llmLog
                            c->top_ids || c->top_logprobs ? c->top : 0u};
     // More rows than SMs: a CTA of 256 threads each, five per SM (2048 rows of 32000 values 50.4 us, 300 rows 14.2; with 512 threads 54.7 and 14.6, with 128
     // and twice the loads 48.6 and 19.6). Else 1024 threads (80 rows 7.3 us against 8.5), and up to 8 CTAs that have 32768 values or more (a row of 32000: one
-    // CTA 10.0 us, two 11.2, four 12.5).
+    // CTA 7.5 us, two 8.9, four 9.5; of 64000: two 10.0, four 9.5, eight 11.0).
     const uint64_t sms = (uint64_t)ctx->sm_count;
     uint32_t peers = 1u;
     while (peers < 8u && peers * 2ull * c->rows <= sms && c->n > 32768u * peers) peers *= 2u;
