@@ -1,8 +1,8 @@
 // Attention of single tokens over a cache in pages: m40llm_attention_paged_async.
 //
-// Work is dealt as (row, kv head, chunk of entries): softmax statistics are kept with a running maximum in base 2, and the chunks'
-// (maximum, sum, unnormalised output) meet in paged_merge_kernel in a fixed order. Where accumulated weights are asked for, the
-// scores are kept in scratch and paged_weights_kernel turns them into weights once the maximum and sum of every row are known.
+// Rows are split over their entries: softmax statistics are kept with a running maximum in base 2, and the parts' (maximum, sum, unnormalised output) meet in a fixed
+// order: in clusters of CTAs for short rows, else in a join behind the kernel that made them. Where accumulated weights are asked for, the scores are kept in scratch
+// and turned into weights once the maximum and sum of every row are known.
 //   paged_tiles_kernel  f16 entries, head sizes 64 and 128: matrix instructions on 64-entry tiles
 //   paged_lanes_kernel  (attention_paged_lanes.cu) f32 entries and other f16 head sizes, rows in 16-byte pieces: f32 multiply-adds in registers
 //   paged_rows_kernel   what is left, odd head sizes and alignments: f32 multiply-adds on tiles in shared memory
@@ -459,7 +459,6 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
             }
         }
         // this thread's entries: e0, e0 + 1, e0 + 8, e0 + 9
-        
         float s[H][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s0[0][i] += s0[1][i], s1[0][i] += s1[1][i];
@@ -531,7 +530,6 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
                 mma16816(o[2 * nd + 1], ph[0][0], pl[0][0], ph[0][1], pl[0][1], b[2], b[3]);
             }
         }
-
         }
         const bool ends = at.tile + 1u == at.tiles;
         if (ends || f + 1u == count) {
