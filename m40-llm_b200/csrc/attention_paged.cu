@@ -648,12 +648,13 @@ __global__ void __launch_bounds__(TILES_THREADS, (TilesCfg<HD, WIDE>::CTAS)) pag
     }
 }
 
-// The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most 1792, the warps of 444 CTAs);
+// The parts of one q head, put together in a fixed order by 256 threads: thread s has the weights of parts s, s + 256, .. (at most PAGED_PARTS_MOST);
 // then 256 / LANES groups of lanes take every so-many-th part, each lane V dimensions, and the groups' sums meet in shared memory. CTAs of 8 lanes share a
 // head's dimensions where there are few heads, for more loads at a time.
 template <int V, int LANES, typename Part>
 __device__ __forceinline__ void paged_join_parts(const PagedAttnArgs& a, size_t head, uint32_t share, uint32_t parts, Part part) {
-    constexpr uint32_t MOST = 1792, GROUPS = 256 / LANES, AT_ONCE = 4;
+    constexpr uint32_t MOST = PAGED_PARTS_MOST, GROUPS = 256 / LANES, AT_ONCE = 4;
+    static_assert(MOST % 256u == 0, "a thread's parts");
     __shared__ float sw[MOST], red[16];
     __shared__ float s_acc[8][LANES * V];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, hd = a.c.hd;
@@ -1021,7 +1022,7 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     const uint32_t shares = (a.group + 15u) / 16u;
     a.heads_at_once = by_lanes ? lanes.heads_at_once : (a.group + shares - 1u) / shares;
     a.part_warps = by_lanes ? lanes.warps : TILES_WARPS;
-    const uint32_t ctas = by_lanes ? lanes.ctas : (uint32_t)ctx->sm_count * (hd == 64u ? TilesCfg<64, false>::CTAS : TilesCfg<128, false>::CTAS);
+    const uint32_t ctas = by_lanes ? lanes.ctas : paged_list_ctas((uint32_t)ctx->sm_count, hd == 64u ? TilesCfg<64, false>::CTAS : TilesCfg<128, false>::CTAS, TILES_WARPS);
     if (!list) {
         const uint64_t work = (uint64_t)c->rows * cache->kv_heads * a.bound, target = 2ull * (uint64_t)ctx->sm_count;
         uint64_t chunk = (work + target - 1) / target;

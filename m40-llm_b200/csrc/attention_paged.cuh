@@ -2,6 +2,7 @@
 #pragma once
 #include "attention_mma.cuh"
 #include "paged.cuh"
+#include "paged_list.cuh"
 
 struct PagedAttnArgs {
     PagedView c;

@@ -307,7 +307,7 @@ bool m40_paged_lanes(const M40llmCudaContext* ctx, const M40llmPagedCache* cache
     // Rings of up to 100 KB and two CTAs on an SM, so that the next launch's CTAs find room as these end: 9 rows of up to 4097 f32 entries 20.0 us, with one CTA of
     // twice the warps 20.9, one row of 64 entries 7.7 against 9.0.
     out->warps = rb <= 512u ? 4u : (rb <= 1024u ? 2u : 1u);
-    out->ctas = 2u * (uint32_t)ctx->sm_count;
+    out->ctas = paged_list_ctas((uint32_t)ctx->sm_count, 2u, out->warps);
     return true;
 }
 

@@ -1,0 +1,13 @@
+// Limits of the list of tiles that attention over a paged cache deals to its resident CTAs. Host arithmetic only.
+#pragma once
+#include <stdint.h>
+
+// Parts of one q head that a join takes: seven of each of its 256 threads. A unit has a part of every warp of the CTAs that touch it, at most of all of them: 444 CTAs
+// of four warps leave 1776.
+constexpr uint32_t PAGED_PARTS_MOST = 1792;
+
+// CTAs that share a list: as many as are resident, but no more than a join takes the parts of. Only devices of 150 SMs or more have fewer at work for it.
+inline uint32_t paged_list_ctas(uint32_t sms, uint32_t per_sm, uint32_t warps) {
+    const uint32_t resident = sms * per_sm, most = PAGED_PARTS_MOST / warps;
+    return resident < most ? resident : most;
+}

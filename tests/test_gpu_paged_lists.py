@@ -1,0 +1,29 @@
+"""Attention over a paged cache where its list of tiles is long: rows that every resident CTA has a part of, and rows over several batches of the list."""
+import numpy as np
+import pytest
+
+import paged_cases as T
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean(nat):
+    yield
+    nat.free_all()
+    T.status(nat)
+
+
+@pytest.mark.parametrize("kind,dim,heads", [("f16", 64, 2), ("f16", 64, 16), ("f16", 128, 4), ("f32", 64, 4), ("f32", 384, 2)])
+@pytest.mark.parametrize("length", [33001, 61000])
+def test_one_row_of_all_ctas(nat, kind, dim, heads, length):
+    """One kv head and one row with a tile or more for every CTA: parts of all warps meet in one join, and in the weights."""
+    rng = np.random.default_rng(dim + heads)
+    c = T.Cache(nat, rng, 1, length + 100, 1, dim, 64, kind)
+    q = (2 * rng.standard_normal((1, heads, dim))).astype(np.float32)
+    got, _ = T.attend(nat, c, q, [0], [length])
+    T.check_attention(c, q, [0], [length], got)
+    w = rng.random((1, 1, c.capacity)).astype(np.float32)
+    got, gw = T.attend(nat, c, q, [0], [length], weights=w, ld=c.capacity, in_place=True)
+    T.check_attention(c, q, [0], [length], got, weights=w, got_w=gw, before=w)
+    assert T.status(nat) == 0

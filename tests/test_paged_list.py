@@ -1,0 +1,48 @@
+"""The list of tiles that attention over a paged cache deals to its CTAs: its limits, compiled by the host compiler or read from the sources. Runs without a GPU."""
+import os
+import re
+import subprocess
+
+import pytest
+
+import helpers
+
+CSRC = os.path.join(helpers.PKG_DIR, "csrc")
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    """Compiles C++ lines that print one number each, and returns those."""
+    def run(lines):
+        folder = tmp_path_factory.mktemp("list")
+        (folder / "ask.cpp").write_text('#include <cstdio>\n#include "%s"\nint main() {\n%s\n}\n' % (os.path.join(CSRC, "paged_list.cuh"), "\n".join(lines)))
+        subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-o", str(folder / "ask"), str(folder / "ask.cpp")], check=True)
+        return [int(x) for x in subprocess.run([str(folder / "ask")], check=True, capture_output=True, text=True).stdout.split()]
+    return run
+
+
+def source(name):
+    return re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+
+
+# CTAs per SM and warps of a CTA, as the kernels' launches have them: heads of 64 and of 128 on tiles, lanes of four, two and one warp
+FORMS = [(3, 4), (2, 4), (2, 2), (2, 1)]
+
+
+@pytest.mark.parametrize("per_sm,warps", FORMS)
+def test_a_join_takes_the_parts_of_all_ctas(ask, per_sm, warps):
+    """One long row of one kv head has a part of every warp of every CTA, whatever the device."""
+    sms = [1, 2, 132, 148, 149, 150, 160, 264, 1000, 100000]
+    most, *ctas = ask(['printf("%u\\n", PAGED_PARTS_MOST);'] + [f'printf("%u\\n", paged_list_ctas({n}, {per_sm}, {warps}));' for n in sms])
+    for n, c in zip(sms, ctas):
+        assert 0 < c * warps <= most and c <= n * per_sm, n
+        assert c == n * per_sm or n >= 150, "all CTAs that are resident, where the join takes them"
+
+
+def test_ctas_of_a_list_are_never_more():
+    """Every number of CTAs goes through that limit, and the join has room for it."""
+    tiles, lanes = source("attention_paged.cu"), source("attention_paged_lanes.cu")
+    assert re.findall(r"\bctas = ([^;]*);", tiles) == [
+        "by_lanes ? lanes.ctas : paged_list_ctas((uint32_t)ctx->sm_count, hd == 64u ? TilesCfg<64, false>::CTAS : TilesCfg<128, false>::CTAS, TILES_WARPS)"]
+    assert re.findall(r"\bctas = ([^;]*);", lanes) == ["paged_list_ctas((uint32_t)ctx->sm_count, 2u, out->warps)"]
+    assert re.search(r"MOST = PAGED_PARTS_MOST\b", tiles) and "sw[MOST]" in tiles
