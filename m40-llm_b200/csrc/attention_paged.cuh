@@ -71,10 +71,10 @@ __device__ __forceinline__ void paged_list_make(const PagedAttnArgs& a, PagedLis
             if (!inside && blockIdx.x == 0) atomicOr(a.status, 1u);
             n = inside && end > begin ? (end - (begin & ~(span - 1u)) + span - 1u) / span : 0u;
         }
-        uint32_t sum = n;  // 32 rows of at most 2^26 tiles
+        uint64_t sum = n;  // 32 rows of 2^30 entries have 2^32 tiles of 8
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, sum, o);
+            const uint64_t u = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= (uint32_t)o) sum += u;
         }
         if (r < rows) {

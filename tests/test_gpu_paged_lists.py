@@ -27,3 +27,19 @@ def test_one_row_of_all_ctas(nat, kind, dim, heads, length):
     got, gw = T.attend(nat, c, q, [0], [length], weights=w, ld=c.capacity, in_place=True)
     T.check_attention(c, q, [0], [length], got, weights=w, got_w=gw, before=w)
     assert T.status(nat) == 0
+
+
+@pytest.mark.parametrize("kind,dim,heads,kv_heads,page", [("f32", 384, 2, 1, 16), ("f16", 64, 8, 2, 16), ("f16", 96, 6, 2, 1)])
+@pytest.mark.parametrize("rows", [31, 32, 33, 64, 97, 256, 300])
+def test_rows_of_several_batches(nat, kind, dim, heads, kv_heads, page, rows):
+    """The tiles before a row are added up 32 rows at a time: rows at the ends of these batches, beside empty ones."""
+    rng = np.random.default_rng(rows + dim)
+    c = T.Cache(nat, rng, 7, 3000, kv_heads, dim, page, kind)
+    slot = np.arange(rows) % 7
+    length = rng.integers(0, 400, rows)
+    length[31::32], length[0::32], length[5] = 700, 0, 2999
+    q = (2 * rng.standard_normal((rows, heads, dim))).astype(np.float32)
+    got, _ = T.attend(nat, c, q, slot, length, max_len=3000)
+    some = np.unique(np.r_[5, np.arange(31, rows, 32), np.arange(30, rows, 32), np.arange(0, rows, 32), np.arange(1, rows, 32), rows - 1])
+    T.check_attention(c, q[some], slot[some], length[some], got[some])
+    assert T.status(nat) == 0

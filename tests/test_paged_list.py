@@ -46,3 +46,13 @@ def test_ctas_of_a_list_are_never_more():
         "by_lanes ? lanes.ctas : paged_list_ctas((uint32_t)ctx->sm_count, hd == 64u ? TilesCfg<64, false>::CTAS : TilesCfg<128, false>::CTAS, TILES_WARPS)"]
     assert re.findall(r"\bctas = ([^;]*);", lanes) == ["paged_list_ctas((uint32_t)ctx->sm_count, 2u, out->warps)"]
     assert re.search(r"MOST = PAGED_PARTS_MOST\b", tiles) and "sw[MOST]" in tiles
+
+
+def test_tiles_before_a_row_do_not_wrap():
+    """32 rows of the most entries that a slot may have, in tiles of one warp's eight: their number takes 33 bits, and so does what is added up over a warp's lanes."""
+    most = 1 << 30
+    assert "> (1ull << 30)" in source("paged.cuh") and 32 * (most // 8) == 1 << 32
+    make = source("attention_paged.cuh")
+    make = make[make.index("void paged_list_make("):make.index("void paged_list_enter(")]
+    added = re.findall(r"(\w+) (?:sum|u|before) =", make)
+    assert len(added) == 3 and set(added) == {"uint64_t"}
