@@ -765,7 +765,8 @@ int m40llm_paged_append_async(M40llmCudaContext* ctx, const M40llmPagedCache* ca
 
 /* Attention of single tokens: out[r] = softmax(scale * q[r] . k) v per q head over the entries row_begin[r] (null: 0) .. row_len[r] - 1 of
  * slot row_slot[r]; q and out f32 [rows][q_heads * head_dim]. A row without entries gives zeros. max_len: a bound of row_len that the
- * work is dealt by (0: the capacity; a row beyond it is one outside the cache).
+ * work is dealt by (0: the capacity; a row beyond it is one outside the cache; M40LLM_ERR_LIMIT where the work of rows of that
+ * length cannot be counted, which takes min(rows, 256) * q_heads * max_len beyond 2^43).
  * With weights_out f32 [slots][kv_heads][ld_weights]: entry e of a slot that has rows in the call, e below the largest row_len of
  * these, gets weights_in[...][e] (null: 0; may be weights_out itself) + the softmax weights that these rows gave it, summed over the q heads of its kv
  * head. Several rows may name the same slot. Other entries stay as they were; so do those of slots with a row outside the cache. Where all of a row's scores are -inf, it gives zeros and no weight. The scores are kept until the sums are known:

@@ -1046,6 +1046,8 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     const uint64_t direct_ctas = (uint64_t)c->rows * units * peers;
     const uint32_t most_tiles = direct_ctas >= ctas ? 32u : (2u * direct_ctas >= ctas ? 16u : 4u);
     const bool direct = tiles && a.bound <= SPAN * peers * most_tiles && direct_ctas <= 0x7fffffffu;
+    const uint32_t span = by_lanes ? 8u * lanes.warps : SPAN;
+    if (list && !direct && !paged_list_fits(c->rows < LIST_ROWS ? c->rows : LIST_ROWS, units, (a.bound + span - 1u) / span, ctas)) return M40LLM_ERR_LIMIT;
     if ((list && !direct) || a.splits > 1 || c->weights_out) {
         a.ld_scores = c->weights_out ? (a.bound + 3u) & ~3u : 0u;
         const size_t rows_at_once = c->rows < LIST_ROWS ? c->rows : LIST_ROWS;
@@ -1072,9 +1074,9 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         e = launch_tiles_of<true>(ctx, a, peers);
         M40_COUNT_LAUNCH(ctx);
     } else if (tiles) {
-        e = launch_list(ctx, a, ctas, SPAN, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x, 1u); });
+        e = launch_list(ctx, a, ctas, span, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return launch_tiles_of<false>(ctx, x, 1u); });
     } else if (by_lanes) {
-        e = launch_list(ctx, a, ctas, 8u * lanes.warps, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
+        e = launch_list(ctx, a, ctas, span, vec_weights, &weighed, [&](const PagedAttnArgs& x) { return m40_paged_lanes_launch(ctx, x, lanes, f32); });
     } else {
         const uint32_t elem = f32 ? 4u : 2u, hd4 = (hd + 3u) & ~3u;
         const uint32_t T = hd4 * elem > 1024u ? 16u : 32u, pitch = ((hd4 * elem + 15u) & ~15u) / elem + 16u / elem;

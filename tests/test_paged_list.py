@@ -56,3 +56,15 @@ def test_tiles_before_a_row_do_not_wrap():
     make = make[make.index("void paged_list_make("):make.index("void paged_list_enter(")]
     added = re.findall(r"(\w+) (?:sum|u|before) =", make)
     assert len(added) == 3 and set(added) == {"uint64_t"}
+
+
+def test_runs_are_counted_in_32_bits(ask):
+    """The longest run of every list that is taken fits, and lists are refused only where it would not."""
+    cases = [(rows, units, tiles, ctas) for rows in (1, 31, 32, 255, 256) for units in (1, 37, 512, 65535) for tiles in (1, 1 << 20, (1 << 27) - 1, 1 << 27)
+             for ctas in (1, 148, 296, 444)]
+    cases += [(1, 1, (1 << 27), 1), (256, 60, 1 << 27, 296), (256, 1, 1 << 24, 1), (256, 1, (1 << 24) - 1, 1)]
+    got = ask([f'printf("%d\\n", paged_list_fits({r}u, {u}ull, {t}u, {c}u));' for r, u, t, c in cases])
+    for (r, u, t, c), fits in zip(cases, got):
+        assert fits == (-(-r * u * t // c) < 1 << 32), (r, u, t, c)
+        assert fits or r * u * t * 8 >> 32 >= c * 8 - 8
+    assert "!paged_list_fits(" in source("attention_paged.cu") and 0 < sum(got) < len(got)
