@@ -996,7 +996,10 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     const uint32_t capacity = paged_capacity(a.c), hd = cache->head_dim;
     if (c->rows == 0 || c->q_heads == 0 || c->q_heads % cache->kv_heads != 0 || c->max_len > capacity) return -2;
     if (c->weights_out && c->ld_weights < capacity) return -2;
-    if (c->rows > 65535u || c->q_heads > 65535u) return M40LLM_ERR_LIMIT;
+    const uint32_t bound = c->max_len ? c->max_len : capacity;
+    const size_t heads = (size_t)c->rows * c->q_heads;
+    // beside the scores, what the parts of fewer than 2^32 rows and heads take is below 2^52 bytes
+    if (c->rows > 65535u || c->q_heads > 65535u || (c->weights_out && heads * bound > PAGED_SCRATCH_MOST / 8u)) return M40LLM_ERR_LIMIT;
     if (m40_ensure_device(ctx) != 0) return -1;
     a.q = (const float*)c->q;
     a.out = (float*)c->out;
@@ -1010,7 +1013,7 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
     a.q_heads = c->q_heads;
     a.group = c->q_heads / cache->kv_heads;
     a.ld_weights = c->ld_weights;
-    a.bound = c->max_len ? c->max_len : capacity;
+    a.bound = bound;
     a.scale = c->scale * LOG2E;
     cudaStream_t s = ctx->decode_stream;
     const bool f32 = cache->elem_dtype == M40LLM_DT_F32;
@@ -1032,7 +1035,6 @@ extern "C" int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llm
         a.chunk = (uint32_t)chunk;
         a.splits = (uint32_t)((a.bound + chunk - 1) / chunk);
     }
-    const size_t heads = (size_t)c->rows * c->q_heads;
     const size_t units = (size_t)cache->kv_heads * ((a.group + a.heads_at_once - 1u) / a.heads_at_once);
     // Short rows: clusters of up to 8 CTAs that fill half of the device take a unit each, without a list and a join. How many tiles a CTA may have then: 32
     // with a wave of CTAs or more, 16 with half of one (the list deals uneven rows better, but its parts and their join cost more the more rows there are), else 4

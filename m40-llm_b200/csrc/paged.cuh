@@ -12,6 +12,7 @@ struct PagedView {
 
 constexpr uint32_t PAGED_NONE = 0xffffffffu;
 constexpr uint32_t PAGED_MAX_HEAD_DIM = 512;
+constexpr size_t PAGED_SCRATCH_MOST = (size_t)1 << 62;  // bytes that a call may ask for before its size could pass 64 bits; what a device has is less
 
 // Page of entry e of a slot, or PAGED_NONE for one outside the pool; the slot and the entry are inside the cache.
 __device__ __forceinline__ uint32_t paged_page(const PagedView& c, uint32_t slot, uint32_t e) {

@@ -636,7 +636,8 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     if (to->kv_heads != cache->kv_heads || to->head_dim != cache->head_dim || to->slots < cache->slots) return -2;
     if (to->k == cache->k && to->table == cache->table && (to->v != cache->v || to->page_tokens != cache->page_tokens || to->max_pages != cache->max_pages)) return -2;
     if (to->elem_dtype != cache->elem_dtype) return -4;
-    if (c->count > 65535u) return M40LLM_ERR_LIMIT;
+    const size_t places = (size_t)c->count * cache->kv_heads * c->keep;  // below 2^62
+    if (c->count > 65535u || places > PAGED_SCRATCH_MOST / 16u) return M40LLM_ERR_LIMIT;
     if (m40_ensure_device(ctx) != 0) return -1;
     // the same pool through the same table is the cache itself
     a.in_place = to->k == cache->k && to->v == cache->v && to->table == cache->table ? 1u : 0u;
@@ -653,7 +654,6 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
     a.recent = c->recent;
     a.ld = c->ld;
     a.bound = c->max_len ? c->max_len : capacity;
-    const size_t places = (size_t)c->count * cache->kv_heads * c->keep;
     uint32_t* work = (uint32_t*)m40_ensure_scratch(ctx, 1, (2 * places + c->count) * sizeof(uint32_t), 0);
     if (!work) return -5;
     a.plan = work;
