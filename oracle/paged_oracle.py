@@ -114,3 +114,14 @@ def logprobs(x, token, top):
         return -np.inf, 0, entropy, lse, ids, tops
     rank = 1 + int(((x > x[token]) | ((x == x[token]) & (np.arange(n) < token))).sum())
     return lp[token], rank, entropy, lse, ids, tops
+
+
+def typical_error(x, K, scale):
+    """What the kernels' 32-bit arithmetic may leave of a head's outputs and weights as a vector, relative to its norm (out_error is for single values, where every rounding
+    points the same way). A score: 8 u of it from x * scale * log2(e), the cut into two f16 parts (2^-22), the factor out of base 2 and the argument of exp2; per
+    step of 16 dimensions the sum so far is cut off at 2 u of it, at its largest here. exp2: 6 u of a weight. Sums: 2 u per 64 entries, 64 u for warps, CTAs and their
+    join. Twice, for outputs (or weights) and the sum that they are divided by."""
+    dim, n = len(x), len(K)
+    steps = np.add.reduceat(K.astype(np.float64) * np.asarray(x, np.float64) * scale, np.arange(0, dim, 16), axis=1)
+    most = np.abs(np.cumsum(steps, axis=1)).max()
+    return 2 * ((2 * -(-dim // 16) + 8) * most + 6 + 2 * n / 64 + 64) * U32
