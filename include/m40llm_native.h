@@ -791,7 +791,9 @@ int m40llm_attention_paged_async(M40llmCudaContext* ctx, const M40llmPagedCache*
  * new_len u32 [count] = min(len, keep). `to` null: in place, only what moves is copied; it may hold pages that no other slot
  * reads. Otherwise the kept entries go to the same slots of `to`, a cache of the same heads, size and type on other pages. new_len may be len. weights_out and
  * entry_pos_out [slots][kv_heads][ld] take the kept entries' values (null: not kept; the arrays themselves: in place).
- * max_len bounds len (0: the capacity). A slot outside the cache or named before in seq, or a length beyond max_len, keeps nothing: new_len 0. */
+ * max_len bounds len (0: the capacity); lists far below it are selected from memory, not from shared memory. first + recent may not pass keep, nor keep the capacity of
+ * either cache, nor max_len that of the source; `ld` is at least the source's (-2 otherwise). A slot outside the cache or named before in seq, or a length beyond max_len,
+ * keeps nothing: new_len 0. */
 typedef struct {
     const M40llmPagedCache* to;
     const uint32_t* seq;
@@ -815,7 +817,7 @@ int m40llm_paged_evict_async(M40llmCudaContext* ctx, const M40llmPagedCache* cac
  * Any output may be null; tokens too where logprob and rank are. NaN counts as -inf, as it does for the greedy choice; values of -inf
  * have probability 0 and are never listed (0xffffffff, -inf in their place). Where a row holds +inf, these share the
  * probability. A row without any value above -inf: entropy 0, lse and logprobs -inf. A token >= n: status bit 8, logprob -inf, rank 0. Decode stream; return
- * codes as above. */
+ * codes as above, M40LLM_ERR_LIMIT for top > 64, n > 2^30 or rows > 2^27. */
 typedef struct {
     const void* logits;
     const uint32_t* tokens;

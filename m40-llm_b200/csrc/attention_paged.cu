@@ -281,7 +281,7 @@ __device__ __forceinline__ bool paged_direct_enter(const PagedAttnArgs& a, Paged
 constexpr uint32_t DIRECT_CLUSTER = 8;
 
 // A run of the list of work per CTA, tiles of 64 entries; a warp takes 16 of them, with a ring of its own. Against one CTA per (row, unit, 1024
-// entries): 32 rows of up to 16384 entries 198 -> 173 us, one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
+// entries): 32 rows of up to 16384 entries 198 -> 173 us (179 to 181 on other B200s), one of 130001 110 -> 90. Runs of single warps spread the reads over four times as many places,
 // and without a barrier per tile the warps drift apart: 187 and 179 us for the 32 rows.
 //   ring      K and V tiles by cp.async, looked up in the page table as they are fetched, XOR-swizzled; it runs on across units.
 //   S = Q K^T, O += P V   mma.sync m16n8k16 with f32 sums. Queries and weights are cut into f16 hi + lo, which leaves 2^-22 of them; a head's query is
